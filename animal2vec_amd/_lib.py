@@ -38,6 +38,13 @@ SIGNATURES = {
     "a2v_attention_dropmask_words": [_i, _i, _i],
     "a2v_attention_bwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _f, _u, _p],
     "a2v_attention_bwd_fused_bias": [_i, _i, _i],
+    "a2v_qk_norm_rope_fwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _f, _i, _i, _i, _i, _i, _p],
+    "a2v_qk_norm_rope_bwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _f, _i, _i, _i, _i, _i, _p, C.c_size_t, _p],
+    "a2v_qk_norm_rope_workspace": [_i, _i, _i, _i, _i],
+    "a2v_linear_attention_fwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _i, _p, C.c_size_t, _p],
+    "a2v_linear_attention_bwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _i, _p, C.c_size_t, _p],
+    "a2v_linear_attention_workspace": [_i, _i, _i, _i, _i, _i, _i, _i],
+    "a2v_linear_attention_step": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p],
     "a2v_layernorm_fwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _ll, _i, _ll, _ll, _f, _i, _f, _u, _p],
     "a2v_layernorm_bwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _ll, _i, _ll, _ll, _i, _f, _u, _i, _p, _p],
     "a2v_instnorm_targets": [_i, C.POINTER(_p), _i, _p, _p, _p, _i, _i, _i, _f, _p],
@@ -91,7 +98,9 @@ ABI12_SIGNATURES = {
 ABI13_SIGNATURES = {
     "a2v_attention_fwd": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _f, _u, _p],
 }
-RESTYPES = {"a2v_query_workspace": C.c_size_t}      # everything else returns int
+# Entries that came without an ABI bump (no signature changed): an older build of ABI 14 lacks them.
+LATER_ENTRIES = tuple(n for n in SIGNATURES if n.startswith(("a2v_qk_norm_rope", "a2v_linear_attention")))
+RESTYPES = {"a2v_query_workspace": C.c_size_t, "a2v_qk_norm_rope_workspace": C.c_size_t, "a2v_linear_attention_workspace": C.c_size_t}      # everything else returns int
 
 _lib = None
 
@@ -126,7 +135,7 @@ def _load_path(path: str, what: str) -> C.CDLL:
         except AttributeError as e:
             # (an older build loaded through A2V_LIB_PATH for a same-box A/B run may predate the ABI-12 entries: ops.py then takes the
             # calls they replaced; the product library must export everything)
-            if name in ABI12_ENTRIES and os.environ.get("A2V_LIB_PATH"):
+            if name in ABI12_ENTRIES + LATER_ENTRIES and os.environ.get("A2V_LIB_PATH"):
                 continue
             raise A2VError(f"{os.path.basename(path)} does not export {name}") from e
         fn.argtypes = argtypes

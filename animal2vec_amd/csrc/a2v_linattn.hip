@@ -1,0 +1,636 @@
+// Linear attention with a decay per head (no softmax; the recurrent counterpart of the ALiBi term): for one head
+//     S_t = l S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,   l = exp(-slope)            S: HD x HD, 32 bits
+// Chunked form over C rows (i, j local to the chunk, Y = l S at its start, "the state as its first row sees it"):
+//     o_i = scale (sum_{j <= i} l^(i-j) (q_i . k_j) v_j + l^i Y^T q_i)
+//     Y'  = l^C Y + sum_j l^(C-j) k_j v_j^T
+// Every power of l is <= 1, so nothing overflows however strong the decay.
+//
+// The backward pass is the same sum three times, with D_t = l D_{t+1} + scale q_t do_t^T running backwards in time:
+//     dq_t = scale S_t do_t    forward in time,  (q, k, v) := (do, v, k),        state S^T
+//     dv_t = D_t^T k_t         backwards,        (q, k, v) := (k, q, scale do),  state D
+//     dk_t = D_t v_t           backwards,        (q, k, v) := (v, scale do, q),  state D^T
+// so ONE kernel does all four: a "role" names its operands, its direction and where the scale goes.
+//
+// One workgroup owns a (sequence, head) or a segment of one and walks its chunks with the state in registers.  A wave owns 16 columns
+// of v: the whole HD x 16 slice of the state lives in its MFMA accumulators, whose layout IS the A operand of Y^T q, so neither the
+// state nor the scores ever pass through LDS; the price is that every wave forms the chunk's scores itself.
+// Products are issued swapped (P^T = K Q^T, O^T = V^T P^T + Y^T Q^T): see a2v_attn.hip for the layout argument.
+//
+// 16-bit runs: scores, the scaled values and the state go into the matrix cores as hi + lo pairs (two products each, 2^-17 relative),
+// because one 16-bit rounding of each would add up to more than the one rounding of the result that the type asks for.
+#include "a2v_common.h"
+
+typedef __attribute__((address_space(3))) s16x4 la_lds_s16x4;
+
+struct LinRole {
+  const void* q; const void* k; const void* v; void* o;
+  long long qn, qs, qh, kn, ks, kh, vn, vs, vh, on, os, oh;     // strides in elements: sequence, row, head
+  int qr, kr, vr;                                                // heads that share one head of the operand
+  int reverse;                                                   // rows are visited from the last to the first
+  int first_t;                                                   // `first` is read transposed
+  int o32;                                                       // o is fp32 whatever the operands are
+  float s_inter, s_state;                                        // factors of Y^T q and of k v^T (their product is the scale)
+  const float* first;                                            // (B, H, HD, HD) state before the first row, or null
+  float* last;                                                   // (B, H, HD, HD) state behind the last row, or null
+  float* ws;                                                     // segment states, slots x H x HD x HD
+};
+struct LinArgs {
+  LinRole r[3];
+  const float* slopes;
+  const int* cu;                                                 // (B + 1) row offsets, or null: B sequences of S rows
+  int B, S, H, T;                                                // T: rows in all (cu), S: rows of a sequence
+  int seg;                                                       // rows of a segment, a multiple of the chunk
+  int slots;                                                     // grid.x / H
+  int fill;                                                      // rows outside every sequence become 0 (cu)
+};
+
+template <typename T> struct LinT;
+template <> struct LinT<bf16> {
+  static constexpr int C = 64, V = 8;                            // rows of a chunk, elements of a 16-byte load
+  static constexpr bool SPLIT = true;
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, const f32x4& c) { return A2V_MFMA_16x16x32(a, b, c, 0, 0, 0); }
+};
+template <> struct LinT<float> {
+  static constexpr int C = 32, V = 4;                            // fp32 MFMA runs at 1/16 of the rate: half the chunk, half the scores
+  static constexpr bool SPLIT = false;
+  struct frag { float e[8]; __device__ __forceinline__ float& operator[](int i) { return e[i]; } __device__ __forceinline__ float operator[](int i) const { return e[i]; } };
+  static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// A tile is C rows of HD elements at a pitch of HD elements + 16 bytes: both the row reads (16 rows, 8 or 16 bytes each) and the
+// transposed reads (4 rows x 32 bytes, or 4 rows x 16 words) then touch every bank once.
+template <typename T, int HD> __device__ __forceinline__ constexpr int lin_pitch() { return HD + 16 / (int)sizeof(T); }
+
+// 8 elements of row `r` at columns {32 kd + 4 g ..+3} and {32 kd + 16 + 4 g ..+3}: the order the state's accumulator tiles have
+template <typename T, int HD> __device__ __forceinline__ typename LinT<T>::frag lin_row(const T* tile, int r, int kd, int g) {
+  const T* p = tile + r * lin_pitch<T, HD>() + 32 * kd + 4 * g;
+  typename LinT<T>::frag f;
+  if constexpr (LinT<T>::SPLIT) {
+    const bf16x4 a = *(const bf16x4*)p, b = *(const bf16x4*)(p + 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[4 + i] = b[i]; }
+  } else {
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[4 + i] = b[i]; }
+  }
+  return f;
+}
+// the transpose: column `c0 + lane % 16`, rows {32 ks + 4 g ..+3} and {32 ks + 16 + 4 g ..+3}
+template <typename T, int HD> __device__ __forceinline__ typename LinT<T>::frag lin_col(const T* tile, int ks, int c0, int lane) {
+  typename LinT<T>::frag f;
+  const int g = lane >> 4;
+  constexpr int P = lin_pitch<T, HD>();
+  if constexpr (LinT<T>::SPLIT) {
+    const T* p = tile + (32 * ks + 4 * g + ((lane & 15) >> 2)) * P + c0 + 4 * (lane & 3);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)(p + 16 * P));
+    union { struct { s16x4 a, b; } s; bf16x8 v; } u;
+    u.s.a = a; u.s.b = b;
+    f = u.v;
+  } else {
+    const T* p = tile + (32 * ks + 4 * g) * P + c0 + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = p[i * P]; f[4 + i] = p[(16 + i) * P]; }
+  }
+  return f;
+}
+template <typename T> __device__ __forceinline__ void lin_split(const float* x, typename LinT<T>::frag& hi, typename LinT<T>::frag& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = (T)x[i];
+    if constexpr (LinT<T>::SPLIT) lo[i] = (T)(x[i] - (float)hi[i]);
+  }
+}
+
+// slot -> (sequence, segment).  Sequences start wherever cu says, so sequence b gets the slots floor(start / seg) + b ...: that many are
+// always enough (ceil(len / seg) <= floor((start + len) / seg) - floor(start / seg) + 1), none is shared, and their number is known to
+// the host without reading cu.  Offsets are clamped to [0, T]: a wrong cu gives wrong rows, never an access outside the tensors.
+struct LinSeq { int b, p, np, begin, len; };                     // begin: first row, len: rows, np: segments
+__device__ __forceinline__ int lin_cu(const LinArgs& a, int b) { const int c = a.cu[b]; return c < 0 ? 0 : (c > a.T ? a.T : c); }
+__device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) {
+  if (!a.cu) {
+    s.np = a.S > a.seg ? (a.S + a.seg - 1) / a.seg : 1;
+    s.b = slot / s.np;
+    s.p = slot - s.b * s.np;
+    s.begin = 0;
+    s.len = a.S;
+    return s.b < a.B;
+  }
+  int lo = 0, hi = a.B;                                          // the last b in [0, B) whose first slot is <= slot
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (lin_cu(a, mid) / a.seg + mid <= slot) lo = mid; else hi = mid;
+  }
+  s.b = lo;
+  s.begin = lin_cu(a, lo);
+  const int end = lin_cu(a, lo + 1);
+  s.len = end > s.begin ? end - s.begin : 0;
+  s.np = s.len > a.seg ? (s.len + a.seg - 1) / a.seg : 1;
+  s.p = slot - (s.begin / a.seg + lo);
+  return s.p >= 0 && s.p < s.np;
+}
+__device__ __forceinline__ float lin_log2(const float* slopes, int h) {
+  const float l2 = -slopes[h] * 1.44269504088896341f;
+  return l2 < -4096.f ? -4096.f : l2;                            // (an infinite slope: l^0 = 1, l^n = 0; NaN stays NaN)
+}
+__device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
+
+// STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
+template <typename T, int HD, bool STATE>
+__global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
+  typedef LinT<T> L;
+  typedef typename L::frag frag;
+  constexpr int C = L::C, NT = C / 16, NS = C / 32, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, P = lin_pitch<T, HD>();
+  constexpr int CPR = HD / L::V;                                 // 16-byte pieces of a row; C * CPR / THREADS = 2 for every T and HD
+  static_assert(C * CPR == 2 * THREADS, "two pieces per thread and tile");
+  __shared__ __attribute__((aligned(16))) T sm[3][C * P];
+  T* const sQ = sm[0];
+  T* const sK = sm[1];
+  T* const sV = sm[2];
+  const LinRole& r = a.r[blockIdx.y];
+  const int slot = blockIdx.x / a.H, h = blockIdx.x - slot * a.H;
+  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, n0 = (tid >> 6) * 16;
+  LinSeq s;
+  const bool mine = lin_find(a, slot, s);
+  T* const oT = (T*)r.o;
+  float* const oF = (float*)r.o;
+  if constexpr (!STATE) {
+    if (a.fill) {                                                // rows in front of the first and behind the last sequence
+      int z0 = 0, z1 = 0;
+      const int c0 = lin_cu(a, 0), cB = lin_cu(a, a.B), behind = slot - (cB / a.seg + a.B);
+      if (behind >= 0) { z0 = cB + behind * a.seg; z1 = z0 + a.seg < a.T ? z0 + a.seg : a.T; }
+      else if (slot <= c0 / a.seg) { z0 = slot * a.seg; z1 = z0 + a.seg < c0 ? z0 + a.seg : c0; }
+      for (long long i = tid; i < (long long)(z1 - z0) * HD; i += THREADS) {
+        const long long at = (z0 + i / HD) * r.os + (long long)h * r.oh + i % HD;
+        if (r.o32) oF[at] = 0.f; else oT[at] = (T)0.f;
+      }
+    }
+  }
+  if (!mine) return;
+  if (STATE && s.p == s.np - 1) return;                          // nothing starts from the last segment's state
+  const int b = s.b;
+  const long long sh = ((long long)b * a.H + h) * HD * HD;
+  const int from = s.p * a.seg, upto = STATE || s.len - from > a.seg ? from + a.seg : s.len;     // visited positions of this segment
+  const bool ends = s.p == s.np - 1;                             // this workgroup meets the sequence's last position
+  const float l2 = lin_log2(a.slopes, h);
+  const int off = r.reverse ? 0 : 1;                             // `first` is S_0 forward (Y = l S_0) and Y itself backwards
+
+  f32x4 S[ND];                                                   // S[t][i]: row 16 t + 4 g + i of the state, column n0 + fr
+#pragma unroll
+  for (int t = 0; t < ND; ++t) S[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if constexpr (!STATE) {
+    if (r.first) {
+      const float f0 = s.len ? lin_pow(l2, from + off) : 1.f;    // an empty sequence hands its state on as it is
+      const float* const p = r.first + sh;
+#pragma unroll
+      for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * t + 4 * g + i;
+          S[t][i] = f0 * (r.first_t ? p[(n0 + fr) * HD + d] : p[d * HD + n0 + fr]);
+        }
+    }
+    if (s.p) {
+      const f32x4* const w = (const f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
+#pragma unroll
+      for (int t = 0; t < ND; ++t) S[t] += w[t * 64];
+    }
+  }
+
+  const T* const q = (const T*)r.q + (a.cu ? 0 : b * r.qn) + (long long)(h / r.qr) * r.qh;
+  const T* const k = (const T*)r.k + (a.cu ? 0 : b * r.kn) + (long long)(h / r.kr) * r.kh;
+  const T* const v = (const T*)r.v + (a.cu ? 0 : b * r.vn) + (long long)(h / r.vr) * r.vh;
+  const int row0 = r.reverse ? s.begin + s.len - 1 : s.begin, dir = r.reverse ? -1 : 1;      // row of position t: row0 + dir * t
+
+  uint4 pq[2], pk[2], pv[2];                                     // the next chunk's tiles, in flight during this one's math
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int c = tid + u * THREADS, t = t0 + c / CPR, e = (c % CPR) * L::V;
+      const uint4 z = {0u, 0u, 0u, 0u};
+      pq[u] = z; pk[u] = z; pv[u] = z;
+      if (t < upto) {
+        const long long row = row0 + dir * t;
+        if constexpr (!STATE) pq[u] = *(const uint4*)(q + row * r.qs + e);
+        pk[u] = *(const uint4*)(k + row * r.ks + e);
+        pv[u] = *(const uint4*)(v + row * r.vs + e);
+      }
+    }
+  };
+  auto place = [&]() {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int c = tid + u * THREADS, at = (c / CPR) * P + (c % CPR) * L::V;
+      if constexpr (!STATE) *(uint4*)(sQ + at) = pq[u];
+      *(uint4*)(sK + at) = pk[u];
+      *(uint4*)(sV + at) = pv[u];
+    }
+  };
+
+  // l^(i - j) scale for a query column fr and key rows 4 g + i: inside a tile, and one tile apart
+  const float scale = r.s_inter * r.s_state;
+  float w0[4], w1[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = fr - 4 * g - i;
+    w0[i] = d < 0 ? 0.f : scale * lin_pow(l2, d);
+    w1[i] = scale * lin_pow(l2, 16 + d);
+  }
+  const float l16 = lin_pow(l2, 16), lrow = r.s_inter * lin_pow(l2, fr);
+
+  if (from < upto) fetch(from);
+  for (int t0 = from; t0 < upto; t0 += C) {
+    const int c = upto - t0 < C ? upto - t0 : C;
+    place();
+    __syncthreads();
+    if (t0 + C < upto) fetch(t0 + C);
+
+    frag vf[NS];
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks) vf[ks] = lin_col<T, HD>(sV, ks, n0, lane);
+    if constexpr (!STATE) {
+      f32x4 acc[NT];
+      {
+        frag sh_[NK], sl_[NK];
+#pragma unroll
+        for (int kd = 0; kd < NK; ++kd) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
+          lin_split<T>(x, sh_[kd], sl_[kd]);
+        }
+        float f = lrow;
+#pragma unroll
+        for (int ti = 0; ti < NT; ++ti) {
+          acc[ti] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kd = 0; kd < NK; ++kd) {
+            const frag qf = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
+            acc[ti] = L::mma(sh_[kd], qf, acc[ti]);
+            if constexpr (L::SPLIT) acc[ti] = L::mma(sl_[kd], qf, acc[ti]);
+          }
+          acc[ti] *= f;
+          f *= l16;
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        frag ka[NK], kb[NK];
+#pragma unroll
+        for (int kd = 0; kd < NK; ++kd) {
+          ka[kd] = lin_row<T, HD>(sK, 32 * ks + fr, kd, g);
+          kb[kd] = lin_row<T, HD>(sK, 32 * ks + 16 + fr, kd, g);
+        }
+        float fa = 1.f, fb = 1.f;                                // l^(16 (tiles between the query's and the key's, less one))
+#pragma unroll
+        for (int ti = 2 * ks; ti < NT; ++ti) {
+          f32x4 pa = (f32x4){0.f, 0.f, 0.f, 0.f}, pb = pa;
+#pragma unroll
+          for (int kd = 0; kd < NK; ++kd) {
+            const frag qf = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
+            pa = L::mma(ka[kd], qf, pa);
+            if (ti > 2 * ks) pb = L::mma(kb[kd], qf, pb);
+          }
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // on the diagonal a select, not a product: a non-finite key does not reach the rows in front of it
+            x[i] = ti == 2 * ks ? (fr < 4 * g + i ? 0.f : pa[i] * w0[i]) : pa[i] * (w1[i] * fa);
+            x[4 + i] = ti == 2 * ks ? 0.f : ti == 2 * ks + 1 ? (fr < 4 * g + i ? 0.f : pb[i] * w0[i]) : pb[i] * (w1[i] * fb);
+          }
+          frag hi, lo;
+          lin_split<T>(x, hi, lo);
+          acc[ti] = L::mma(vf[ks], hi, acc[ti]);
+          if constexpr (L::SPLIT) acc[ti] = L::mma(vf[ks], lo, acc[ti]);
+          if (ti > 2 * ks) { fb = fa; fa *= l16; }
+        }
+      }
+#pragma unroll
+      for (int ti = 0; ti < NT; ++ti) {
+        const int t = t0 + 16 * ti + fr;
+        if (t < upto) {
+          const long long at = (a.cu ? 0 : b * r.on) + (long long)(row0 + dir * t) * r.os + (long long)h * r.oh + n0 + 4 * g;
+          if (r.o32) *(f32x4*)(oF + at) = acc[ti];
+          else Vec4<T>::store(oT + at, acc[ti]);
+        }
+      }
+    }
+    const bool last = ends && t0 + C >= upto;
+    if (!last || r.last) {
+      const int e = last ? c - off : c;                          // the state behind the last row itself, or as the next row sees it
+      const float le = lin_pow(l2, e);
+#pragma unroll
+      for (int t = 0; t < ND; ++t) S[t] *= le;
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = e - (32 * ks + 16 * (i >> 2) + 4 * g + (i & 3));
+          x[i] = (float)vf[ks][i] * (r.s_state * lin_pow(l2, n < 0 ? 0 : n));        // rows behind the end hold 0
+        }
+        frag hi, lo;
+        lin_split<T>(x, hi, lo);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          const frag kf = lin_col<T, HD>(sK, ks, 16 * t, lane);
+          S[t] = L::mma(kf, hi, S[t]);
+          if constexpr (L::SPLIT) S[t] = L::mma(kf, lo, S[t]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (STATE) {
+    f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
+#pragma unroll
+    for (int t = 0; t < ND; ++t) w[t * 64] = S[t];
+  } else if (ends && r.last) {
+    float* const p = r.last + sh;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[(16 * t + 4 * g + i) * HD + n0 + fr] = S[t][i];
+  }
+}
+
+// ws[slot] := the state in front of segment p from the segments before it: carried through the sequence's slots in order, one thread per
+// four elements (any order of them: the waves' register image).  The part of `first` is added by the kernel that starts from it.
+__global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
+  const int b = blockIdx.y;
+  LinSeq s;
+  if (a.cu) {
+    s.begin = lin_cu(a, b);
+    const int end = lin_cu(a, b + 1);
+    s.len = end > s.begin ? end - s.begin : 0;
+  } else { s.begin = 0; s.len = a.S; }
+  s.np = s.len > a.seg ? (s.len + a.seg - 1) / a.seg : 1;
+  if (s.np < 2) return;
+  const int slot0 = a.cu ? s.begin / a.seg + b : b * s.np;
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;       // element of (H, HD, HD); HD * HD % 1024 == 0
+  const int h = (int)(i / HH);
+  const float f = lin_pow(lin_log2(a.slopes, h), a.seg);
+  f32x4* w = (f32x4*)(a.r[blockIdx.z].ws + (long long)slot0 * a.H * HH + i);
+  const long long step = (long long)a.H * HH / 4;
+  f32x4 carry = {0.f, 0.f, 0.f, 0.f};
+  int p = 0;
+  for (; p + 4 < s.np; p += 4) {                                 // four loads in flight (the last segment has no state of its own)
+    f32x4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = w[(p + u) * step];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { w[(p + u) * step] = carry; carry = carry * f + x[u]; }
+  }
+  for (; p < s.np - 1; ++p) { const f32x4 x = w[p * step]; w[p * step] = carry; carry = carry * f + x; }
+  w[p * step] = carry;
+}
+
+// the gradients of a shared k / v head: the sum over its heads, of fp32 rows (T, H, HD) -> rows of HK heads
+template <typename T>
+__global__ __launch_bounds__(256) void lin_join_kernel(const float* dk32, const float* dv32, T* dk, T* dv, long long kn, long long ks, long long kh,
+                                                       long long vn, long long vs, long long vh, const int* cu, int B, int S, int T_, int H, int rep, int HD, int fill) {
+  const int HK = H / rep, per = HK * HD / 4;
+  const long long rows = cu ? T_ : (long long)B * S, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const long long row = i / per;
+  const int e = (int)(i - row * per) * 4, hk = e / HD, d = e - hk * HD;
+  const long long n = cu ? 0 : row / S, t = cu ? row : row - n * S;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, c = a;
+  const bool in = !cu || (t >= cu[0] && t < cu[B]);
+  if (!in && !fill) return;
+  if (in) {
+    const float* p = dk32 + (row * H + hk * rep) * HD + d;
+    const float* q = dv32 + (row * H + hk * rep) * HD + d;
+    for (int u = 0; u < rep; ++u) { a += *(const f32x4*)(p + u * HD); c += *(const f32x4*)(q + u * HD); }
+  }
+  Vec4<T>::store(dk + n * kn + t * ks + hk * kh + d, a);
+  Vec4<T>::store(dv + n * vn + t * vs + hk * vh + d, c);
+}
+
+// One token of each of N streams, the state updated in place: state once in, once out, everything else is negligible (HBM, or latency
+// where N H is small).  A thread holds four neighbouring columns of HD * HD / 1024 rows of the state.
+// slots[n] names the state of row n.  Rows that name the same slot are successive tokens of one stream, in row order: the workgroup of
+// the first of them takes them all (the others find an earlier row and leave), so there is no race and no order left open.  A slot
+// outside [0, n_slots) leaves every state alone and gives a row of zeros (padding rows of a captured graph).
+struct LinStep {
+  const void* q; const void* k; const void* v; void* o;
+  long long qn, qh, kn, kh, vn, vh, on, oh;
+  const float* slopes; float* state; const int* slots;
+  int n_slots, N, H, rep;
+  float scale;
+};
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void lin_step_kernel(LinStep a) {
+  constexpr int LPR = HD / 4, RPP = 256 / LPR, NP = HD / RPP;    // lanes of a row, rows of a pass, passes
+  __shared__ f32x4 part[4 * LPR];
+  const int n = blockIdx.x / a.H, h = blockIdx.x - n * a.H, tid = threadIdx.x, hk = h / a.rep;
+  const int c = (tid % LPR) * 4, r0 = tid / LPR;
+  const int slot = a.slots ? a.slots[n] : n;
+  T* const out = (T*)a.o + h * a.oh;
+  if (slot < 0 || slot >= a.n_slots) {
+    if (tid < LPR) Vec4<T>::store(out + n * a.on + c, (f32x4){0.f, 0.f, 0.f, 0.f});
+    return;
+  }
+  float* const st = a.state + ((long long)slot * a.H + h) * HD * HD;
+  f32x4 S[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) S[p] = *(const f32x4*)(st + (r0 + p * RPP) * HD + c);
+  bool more = false;
+  if (a.slots) {
+    bool before = false;
+    for (int m = tid; m < a.N; m += 256)
+      if (a.slots[m] == slot) { before |= m < n; more |= m > n; }
+    if (__syncthreads_or(before)) return;
+    more = __syncthreads_or(more);
+  }
+  const float l = lin_pow(lin_log2(a.slopes, h), 1);
+  for (int m = n; m < a.N; ++m) {
+    if (m > n && a.slots[m] != slot) continue;
+    const T* const q = (const T*)a.q + m * a.qn + h * a.qh;
+    const T* const k = (const T*)a.k + m * a.kn + hk * a.kh;
+    const f32x4 v = Vec4<T>::load((const T*)a.v + m * a.vn + hk * a.vh + c);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int d = r0 + p * RPP;
+      S[p] = S[p] * l + v * ldf(k + d);
+      o += S[p] * ldf(q + d);
+    }
+#pragma unroll
+    for (int x = LPR; x < 64; x <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+    if ((tid & 63) < LPR) part[(tid >> 6) * LPR + (tid & 63)] = o;
+    __syncthreads();
+    if (tid < LPR) Vec4<T>::store(out + m * a.on + c, (part[tid] + part[LPR + tid] + part[2 * LPR + tid] + part[3 * LPR + tid]) * a.scale);
+    if (!more) break;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int p = 0; p < NP; ++p) *(f32x4*)(st + (r0 + p * RPP) * HD + c) = S[p];
+}
+
+// ------------------------------------------------------------------------------------------------------------------ host side
+#define LIN_WGS 1024          /* workgroups that fill the card: four on each of 256 CUs */
+
+// Rows of a segment.  Enough (sequence, head) pairs: one segment each, k and v read once.  Fewer: the axis is cut until LIN_WGS
+// workgroups run, which costs a second pass over k and v; not below 4 HD rows, where the states (HD * HD * 4 bytes, written and read)
+// would weigh as much as those rows.
+static int lin_seg(int B, long long rows, int S, int H, int HD, bool packed, int C) {
+  const long long all = packed ? rows : S;
+  if (!packed && (long long)B * H >= LIN_WGS / 2) return all > 0 ? cdiv(all, C) * C : C;
+  long long seg = (rows * H + LIN_WGS - 1) / LIN_WGS;
+  if (seg < 4 * HD) seg = 4 * HD;
+  if (seg > all) seg = all;
+  return seg < C ? C : cdiv(seg, C) * C;
+}
+struct LinPlan { int C, seg, slots; bool split; size_t states; };
+static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPlan& p) {
+  p.C = dtype == A2V_F32 ? LinT<float>::C : LinT<bf16>::C;
+  const long long rows = packed ? S : (long long)B * S;
+  if (rows >= (1LL << 30)) return false;
+  p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
+  const long long slots = packed ? (long long)S / p.seg + B + 1 : (long long)B * (S > p.seg ? (S + p.seg - 1) / p.seg : 1);
+  if (slots * H >= (1LL << 31)) return false;
+  p.slots = (int)slots;
+  p.split = S > p.seg;
+  p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
+  return true;
+}
+static bool lin_shape_ok(int B, int S, int H, int HK, int HD) {
+  return B >= 0 && S >= 0 && H > 0 && HK > 0 && H % HK == 0 && H <= 65535 && B <= 65535 * 16 && (HD == 32 || HD == 64 || HD == 128);
+}
+static bool lin_tensor_ok(const void* p, const long long* st, int es) {
+  return p && !((uintptr_t)p & 15) && !((st[0] * es) & 15) && !((st[1] * es) & 15) && !((st[2] * es) & 15);
+}
+
+template <typename T, int HD>
+static void lin_launch_hd(const LinArgs& a, const LinPlan& p, int roles, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.slots * (long long)a.H), roles), block(HD * 4);
+  if (p.split) {
+    hipLaunchKernelGGL((lin_kernel<T, HD, true>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL(lin_scan_kernel, dim3(a.H * HD * HD / 1024, a.B, roles), dim3(256), 0, stream, a, HD * HD);
+  }
+  hipLaunchKernelGGL((lin_kernel<T, HD, false>), grid, block, 0, stream, a);
+}
+template <typename T>
+static void lin_launch(const LinArgs& a, const LinPlan& p, int roles, int HD, hipStream_t stream) {
+  if (HD == 32) lin_launch_hd<T, 32>(a, p, roles, stream);
+  else if (HD == 64) lin_launch_hd<T, 64>(a, p, roles, stream);
+  else lin_launch_hd<T, 128>(a, p, roles, stream);
+}
+static int lin_dtype(int dtype) {
+  if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
+#ifdef A2V_ELT_F16
+  if (dtype == A2V_BF16) return A2V_ERR_UNSUPPORTED;             // states and scores have bf16's range, not half's (65504)
+#endif
+  return A2V_OK;
+}
+
+extern "C" size_t a2v_linear_attention_workspace(int dtype, int backward, int packed, int B, int S, int H, int HK, int HD) {
+  LinPlan p;
+  if (!lin_shape_ok(B, S, H, HK, HD) || !lin_plan(dtype, B, S, H, HD, packed != 0, p)) return 0;
+  const size_t rows = packed ? (size_t)S : (size_t)B * S;
+  return (backward ? 3 : 1) * p.states + (backward && H != HK ? 2 * rows * H * HD * sizeof(float) : 0);
+}
+
+extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides,
+                                        const float* slopes, const float* state, float* state_out, const int* cu_seqlens, int B, int S, int H,
+                                        int HK, int HD, float scale, int zero_outside, void* ws, size_t ws_bytes, hipStream_t stream) {
+  if (int e = lin_dtype(dtype)) return e;
+  LinPlan p;
+  if (!strides || !slopes || !lin_shape_ok(B, S, H, HK, HD) || !lin_plan(dtype, B, S, H, HD, cu_seqlens != nullptr, p)) return A2V_ERR_ARG;
+  if (B == 0) return A2V_OK;                                     // no sequence: nothing is read or written
+  const int es = dtype == A2V_F32 ? 4 : 2;
+  if (S > 0 && !(lin_tensor_ok(q, strides, es) && lin_tensor_ok(k, strides + 3, es) && lin_tensor_ok(v, strides + 6, es) && lin_tensor_ok(out, strides + 9, es)))
+    return A2V_ERR_ARG;
+  if (p.states > ws_bytes || (p.states && (!ws || ((uintptr_t)ws & 15)))) return A2V_ERR_ARG;
+  LinArgs a;
+  a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
+  LinRole& r = a.r[0];
+  r = LinRole{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10],
+              strides[11], 1, H / HK, H / HK, 0, 0, 0, scale, 1.f, state, state_out, (float*)ws};
+  a.r[1] = a.r[2] = r;
+  if (dtype == A2V_F32) lin_launch<float>(a, p, 1, HD, stream);
+  else lin_launch<bf16>(a, p, 1, HD, stream);
+  A2V_CHECK_LAUNCH();
+  return A2V_OK;
+}
+
+extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k, const void* v, const void* d_out, void* dq, void* dk, void* dv,
+                                        const long long* strides, const float* slopes, const float* state, const float* d_state_out, float* d_state,
+                                        const int* cu_seqlens, int B, int S, int H, int HK, int HD, float scale, int zero_outside, void* ws,
+                                        size_t ws_bytes, hipStream_t stream) {
+  if (int e = lin_dtype(dtype)) return e;
+  LinPlan p;
+  if (!strides || !slopes || !lin_shape_ok(B, S, H, HK, HD) || !lin_plan(dtype, B, S, H, HD, cu_seqlens != nullptr, p)) return A2V_ERR_ARG;
+  if (B == 0) return A2V_OK;                                     // no sequence: nothing is read or written
+  const int es = dtype == A2V_F32 ? 4 : 2, rep = H / HK;
+  const void* const t[7] = {q, k, v, d_out, dq, dk, dv};
+  if (S > 0)
+    for (int i = 0; i < 7; ++i)
+      if (!lin_tensor_ok(t[i], strides + 3 * i, es)) return A2V_ERR_ARG;
+  const size_t need = a2v_linear_attention_workspace(dtype, 1, cu_seqlens != nullptr, B, S, H, HK, HD);
+  if (need > ws_bytes || (need && (!ws || ((uintptr_t)ws & 15)))) return A2V_ERR_ARG;
+  char* w = (char*)ws;
+  const size_t rows = cu_seqlens ? (size_t)S : (size_t)B * S;
+  float* const dk32 = (float*)(w + 3 * p.states);
+  float* const dv32 = dk32 + rows * H * HD;
+  const long long* const s = strides;
+  const long long pn = (long long)S * H * HD, ps = (long long)H * HD;
+  LinArgs a;
+  a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
+  a.r[0] = LinRole{d_out, v, k, dq, s[9], s[10], s[11], s[6], s[7], s[8], s[3], s[4], s[5], s[12], s[13], s[14],
+                   1, rep, rep, 0, 1, 0, scale, 1.f, state, nullptr, (float*)w};
+  a.r[1] = LinRole{k, q, d_out, dv, s[3], s[4], s[5], s[0], s[1], s[2], s[9], s[10], s[11], s[18], s[19], s[20],
+                   rep, 1, 1, 1, 0, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
+  a.r[2] = LinRole{v, d_out, q, dk, s[6], s[7], s[8], s[9], s[10], s[11], s[0], s[1], s[2], s[15], s[16], s[17],
+                   rep, 1, 1, 1, 1, 0, 1.f, scale, d_state_out, nullptr, (float*)(w + 2 * p.states)};
+  if (rep > 1) {
+    LinRole* const g[2] = {&a.r[1], &a.r[2]};
+    float* const to[2] = {dv32, dk32};
+    for (int i = 0; i < 2; ++i) { g[i]->o = to[i]; g[i]->on = pn; g[i]->os = ps; g[i]->oh = HD; g[i]->o32 = 1; }
+  }
+  if (dtype == A2V_F32) lin_launch<float>(a, p, 3, HD, stream);
+  else lin_launch<bf16>(a, p, 3, HD, stream);
+  if (rep > 1 && rows) {
+    const dim3 grid((unsigned)cdiv((long)(rows * HK * HD / 4), 256));
+    if (dtype == A2V_F32)
+      hipLaunchKernelGGL(lin_join_kernel<float>, grid, dim3(256), 0, stream, dk32, dv32, (float*)dk, (float*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
+                         cu_seqlens, B, S, S, H, rep, HD, a.fill);
+    else
+      hipLaunchKernelGGL(lin_join_kernel<bf16>, grid, dim3(256), 0, stream, dk32, dv32, (bf16*)dk, (bf16*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
+                         cu_seqlens, B, S, S, H, rep, HD, a.fill);
+  }
+  A2V_CHECK_LAUNCH();
+  return A2V_OK;
+}
+
+extern "C" int a2v_linear_attention_step(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides,
+                                         const float* slopes, float* state, const int* slots, int n_slots, int N, int H, int HK, int HD, float scale,
+                                         hipStream_t stream) {
+  if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
+  if (!strides || !slopes || !state || ((uintptr_t)state & 15) || N < 0 || H <= 0 || HK <= 0 || H % HK || (HD != 32 && HD != 64 && HD != 128) ||
+      n_slots < (slots ? 0 : N) || (long long)N * H >= (1LL << 31))
+    return A2V_ERR_ARG;
+  if (N == 0) return A2V_OK;
+  const int es = dtype == A2V_F32 ? 4 : 2;
+  const void* const t[4] = {q, k, v, out};
+  for (int i = 0; i < 4; ++i)
+    if (!t[i] || ((uintptr_t)t[i] & (4 * es - 1)) || strides[2 * i] % 4 || strides[2 * i + 1] % 4) return A2V_ERR_ARG;
+  const LinStep a{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
+                  slopes, state, slots, n_slots, N, H, H / HK, scale};
+  const dim3 grid((unsigned)(N * H)), block(256);
+#define LIN_STEP(T_, HD_) hipLaunchKernelGGL((lin_step_kernel<T_, HD_>), grid, block, 0, stream, a)
+  if (dtype == A2V_F32) { if (HD == 32) LIN_STEP(float, 32); else if (HD == 64) LIN_STEP(float, 64); else LIN_STEP(float, 128); }
+  else { if (HD == 32) LIN_STEP(bf16, 32); else if (HD == 64) LIN_STEP(bf16, 64); else LIN_STEP(bf16, 128); }
+#undef LIN_STEP
+  A2V_CHECK_LAUNCH();
+  return A2V_OK;
+}

@@ -555,6 +555,280 @@ def attention_bwd(qkv, out, d_out, lse, pos, slopes, alibi_scale, H, dalibi, dro
 
 
 # ----------------------------------------------------------------------------------------------
+#                       norm + rotation of q and k, linear attention (long recordings, streams)
+# ----------------------------------------------------------------------------------------------
+LIN_HEAD_DIMS = (32, 64, 128)
+
+
+def rope_inv_freq(sections, base=10000.0, device="cuda"):
+    """fp32 radians per position of every channel pair: base^(-i / n) for pair i of an axis of n pairs.  sections: pairs per axis."""
+    return torch.cat([base ** (-torch.arange(n, dtype=torch.float64) / max(1, n)) for n in sections]).float().to(device)
+
+
+def _on_device(fn, args, t, what):
+    """fn(*args, stream) on the current stream of t's device, which need not be the current device"""
+    if t.device.index == torch.cuda.current_device():
+        check(fn(*args, stream()), what)
+    else:
+        with torch.cuda.device(t.device):
+            check(fn(*args, stream()), what)
+
+
+def _heads(what, t, dims, like=None, out=False):
+    """the checks a tensor of heads (..., heads, HD) has to pass: type, unit channel stride, 16-byte rows (include/a2v.h)"""
+    if t.dim() != dims:
+        raise ValueError(f"{what}: {dims} dimensions expected, got shape {tuple(t.shape)}")
+    dt(t)
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise TypeError(f"{what}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    if t.shape[-1] not in LIN_HEAD_DIMS:
+        raise ValueError(f"{what}: head dimension {t.shape[-1]} (built: {LIN_HEAD_DIMS})")
+    if t.numel() == 0:
+        return
+    st, per = t.stride(), per16(t)
+    if st[-1] != 1 or any(s % per for s, n in zip(st[:-1], t.shape) if n > 1) or t.data_ptr() % 16:
+        raise ValueError(f"{what}: the channels of a head must be contiguous and every head start on 16 bytes, got strides {st}")
+    if out and any(s < t.shape[-1] for s, n in zip(st[:-1], t.shape) if n > 1):
+        raise ValueError(f"{what}: an output may not repeat memory, got strides {st}")
+
+
+def _results(what, named, out=True):
+    for n, t, like in named:
+        _heads(f"{what}: {n}", t, like.dim(), like, out=out)
+        if t.shape != like.shape:
+            raise ValueError(f"{what}: {n} {tuple(t.shape)}, expected {tuple(like.shape)}")
+
+
+def _f32(what, t, shape, like):
+    if t.dtype != torch.float32 or t.device != like.device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous float32 {tuple(shape)} on {like.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _overlap(a, b):
+    """whether two tensors of heads may share an element: exact for slots of one packed buffer (equal row strides), else by address range"""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    es = a.element_size()
+    ext = [sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 for t in (a, b)]
+    d = (a.data_ptr() - b.data_ptr()) // es
+    if d >= ext[1] or -d >= ext[0]:
+        return False
+    rows = [s for n, s in zip(a.shape[:-2], a.stride()) if n > 1]
+    if a.shape[:-2] != b.shape[:-2] or rows != [s for n, s in zip(b.shape[:-2], b.stride()) if n > 1] or not rows or min(rows) <= 0 or any(s % min(rows) for s in rows):
+        return True
+    wide = [(t.shape[-2] - 1) * t.stride(-2) + t.shape[-1] for t in (a, b)]          # what a row of each covers, compared modulo the row pitch
+    d %= min(rows)
+    return d < wide[1] or min(rows) - d < wide[0]
+
+
+def _apart(what, outs, ins, inplace=()):
+    """no output shares memory with an input or another output; output i may be inplace[i] itself"""
+    for i, o in enumerate(outs):
+        for t in ins:
+            me = inplace[i] if i < len(inplace) else None
+            if t is me and o.data_ptr() == t.data_ptr() and all(x == y or n == 1 for x, y, n in zip(o.stride(), t.stride(), o.shape)):
+                continue
+            if _overlap(o, t):
+                raise ValueError(f"{what}: an output overlaps an input")
+        if any(_overlap(o, t) for t in outs[i + 1:]):
+            raise ValueError(f"{what}: two outputs overlap")
+
+
+def _strides(*ts):
+    """(sequence, row, head) strides of each tensor as a host array (a dimension of one row counts as 0: it is never stepped along)"""
+    return (C.c_longlong * (3 * len(ts)))(*[s if n > 1 else 0 for t in ts for s, n in zip(t.stride()[:3], t.shape)])
+
+
+def _qk_norm_rope_args(what, q, k, q_weight, k_weight, inv_freq, pos, sections):
+    _heads(f"{what}: q", q, 4)
+    _heads(f"{what}: k", k, 4, q)
+    N, S, H, HD = q.shape
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != HD or H < 1 or k.shape[2] < 1:
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} do not belong together")
+    _f32(f"{what}: q_weight", q_weight, (HD,), q)
+    _f32(f"{what}: k_weight", k_weight, (HD,), q)
+    half = inv_freq.numel()
+    _f32(f"{what}: inv_freq", inv_freq, (half,), q)
+    sections = (half,) if sections is None else tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 3 or min(sections) < 0 or sum(sections) != half or half % 8 or not 8 <= half <= HD // 2:
+        raise ValueError(f"{what}: sections {sections} over {half} frequencies (a multiple of 8, at most half of {HD} channels; 1 to 3 axes)")
+    if pos is None:
+        if len(sections) != 1:
+            raise ValueError(f"{what}: {len(sections)} axes need positions")
+        ps = None
+    else:
+        want = (N, S) if len(sections) == 1 and pos.dim() == 2 else (N, S, len(sections))
+        if pos.dtype != torch.int32 or pos.device != q.device or tuple(pos.shape) != want or (pos.dim() == 3 and pos.shape[2] > 1 and pos.stride(2) != 1):
+            raise ValueError(f"{what}: pos int32 {want} on {q.device} expected, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
+        ps = (C.c_longlong * 2)(*pos.stride()[:2])
+    return inv_freq, pos, ps, len(sections), (C.c_int * len(sections))(*sections)
+
+
+def qk_norm_rope_fwd(q, k, q_weight, k_weight, inv_freq, pos=None, *, sections=None, interleaved=False, eps=1e-6, q_out=None, k_out=None):
+    """q (N,S,H,HD), k (N,S,HK,HD) -> R(pos) (x / sqrt(mean x^2 + eps) * weight) of each head, rounded once.
+
+    q and k may be views of a packed (N,S,3,H,HD) projection; q_out / k_out may be q / k themselves (in place) or other views.
+    q_weight, k_weight (HD) fp32.  inv_freq (half,) fp32: radians per position of each of the `half` channel pairs (rope_inv_freq):
+    (p, p + half), or (2p, 2p + 1) with interleaved=True; half is a multiple of 8 and at most HD / 2, the channels from 2 half on are
+    only normalised.  sections: pairs per axis of the position (one to three axes: time, microphone, band ...), default one axis.
+    pos int32 (N,S) or (N,S,axes), any sign, exact to 32 bits; None: the row's index."""
+    args = _qk_norm_rope_args("qk_norm_rope_fwd", q, k, q_weight, k_weight, inv_freq, pos, sections)
+    N, S, H, HD = q.shape
+    given = q_out is not None or k_out is not None
+    if q_out is None:
+        q_out = _E(N, S, H, HD, dtype=q.dtype, device=q.device)
+    if k_out is None:
+        k_out = _E(N, S, k.shape[2], HD, dtype=q.dtype, device=q.device)
+    if given:
+        _results("qk_norm_rope_fwd", (("q_out", q_out, q), ("k_out", k_out, k)))
+        _apart("qk_norm_rope_fwd", (q_out, k_out), (q, k), (q, k))
+    if q.numel() == 0:
+        return q_out, k_out
+    _on_device(_L().a2v_qk_norm_rope_fwd,
+               (dt(q), ptr(q), ptr(k), ptr(q_out), ptr(k_out), _strides(q, k, q_out, k_out), ptr(q_weight), ptr(k_weight), ptr(args[0]), ptr(args[1]),
+                *args[2:], 1 if interleaved else 0, float(eps), N, S, H, k.shape[2], HD), q, "a2v_qk_norm_rope_fwd")
+    return q_out, k_out
+
+
+def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, inv_freq, pos=None, *, dq_weight, dk_weight, sections=None, interleaved=False,
+                     eps=1e-6, dq=None, dk=None):
+    """-> dq, dk, from the gradients of qk_norm_rope_fwd's results and its inputs (q and k as they were before an in-place call).
+    dq_weight, dk_weight (HD) fp32 are accumulated, in the same order every time.  dq / dk may be dq_out / dk_out themselves."""
+    args = _qk_norm_rope_args("qk_norm_rope_bwd", q, k, q_weight, k_weight, inv_freq, pos, sections)
+    N, S, H, HD = q.shape
+    HK = k.shape[2]
+    _results("qk_norm_rope_bwd", (("dq_out", dq_out, q), ("dk_out", dk_out, k)), out=False)
+    given = dq is not None or dk is not None
+    if dq is None:
+        dq = _E(N, S, H, HD, dtype=q.dtype, device=q.device)
+    if dk is None:
+        dk = _E(N, S, HK, HD, dtype=q.dtype, device=q.device)
+    _f32("qk_norm_rope_bwd: dq_weight", dq_weight, (HD,), q)
+    _f32("qk_norm_rope_bwd: dk_weight", dk_weight, (HD,), q)
+    if dq_weight.data_ptr() == dk_weight.data_ptr():
+        raise ValueError("qk_norm_rope_bwd: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
+    if given:
+        _results("qk_norm_rope_bwd", (("dq", dq, q), ("dk", dk, k)))
+        _apart("qk_norm_rope_bwd", (dq, dk), (dq_out, dk_out, q, k), (dq_out, dk_out))
+    if q.numel() == 0:
+        return dq, dk
+    need = _L().a2v_qk_norm_rope_workspace(N, S, H, HK, HD)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _on_device(_L().a2v_qk_norm_rope_bwd,
+               (dt(q), ptr(dq_out), ptr(dk_out), ptr(q), ptr(k), ptr(dq), ptr(dk), _strides(dq_out, dk_out, q, k, dq, dk), ptr(q_weight), ptr(k_weight),
+                ptr(dq_weight), ptr(dk_weight), ptr(args[0]), ptr(args[1]), *args[2:], 1 if interleaved else 0, float(eps), N, S, H, HK, HD, ptr(ws), need), q, "a2v_qk_norm_rope_bwd")
+    return dq, dk
+
+
+def _linear_attention_args(what, q, k, v, slopes, state, cu_seqlens):
+    if _HALF and q.dtype == torch.float16:
+        raise TypeError(f"{what}: not built for float16 (a state does not fit its range); use bfloat16 or float32")
+    _heads(f"{what}: q", q, 4)
+    _heads(f"{what}: k", k, 4, q)
+    _heads(f"{what}: v", v, 4, q)
+    N, S, H, HD = q.shape
+    if k.shape != v.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != HD or H < 1 or k.shape[2] < 1 or H % k.shape[2]:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    _f32(f"{what}: slopes", slopes, (H,), q)
+    B = N
+    if cu_seqlens is not None:
+        if N != 1 or cu_seqlens.dtype != torch.int32 or cu_seqlens.device != q.device or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous():
+            raise ValueError(f"{what}: cu_seqlens needs one row of packed sequences (N = 1) and int32 offsets (sequences + 1,) on {q.device}")
+        B = cu_seqlens.numel() - 1
+    if state is not None:
+        _f32(f"{what}: state", state, (B, H, HD, HD), q)
+    return B, S, H, k.shape[2], HD
+
+
+def linear_attention_fwd(q, k, v, slopes, *, scale=None, state=None, cu_seqlens=None, out=None, want_state=False):
+    """S_t = exp(-slopes[h]) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t  -> out (N,S,H,HD), state behind the last row or None.
+
+    q (N,S,H,HD), k, v (N,S,HK,HD) bf16 or fp32, views of a packed projection among them; HK divides H.  slopes (H) fp32 >= 0.
+    scale: default HD^-0.5.  state (B,H,HD,HD) fp32: what the sequences start from (None: nothing), never changed.
+    cu_seqlens (B+1) int32 on the device: q, k, v are (1,T,heads,HD) and sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1], which may
+    be none; rows outside every sequence are zeros in a result of this call's own and left as they were in the caller's `out`.
+    The products take 16-bit operands as pairs: sums, scores and states keep fp32 accuracy, out is rounded once."""
+    B, S, H, HK, HD = _linear_attention_args("linear_attention_fwd", q, k, v, slopes, state, cu_seqlens)
+    own = out is None
+    if own:
+        out = _E(*q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _results("linear_attention_fwd", (("out", out, q),))
+        _apart("linear_attention_fwd", (out,), (q, k, v))
+    last = _E(B, H, HD, HD, dtype=torch.float32, device=q.device) if want_state else None
+    if B == 0:
+        return out, last
+    need = _L().a2v_linear_attention_workspace(dt(q), 0, cu_seqlens is not None, B, S, H, HK, HD)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _on_device(_L().a2v_linear_attention_fwd,
+               (dt(q), ptr(q), ptr(k), ptr(v), ptr(out), _strides(q, k, v, out), ptr(slopes), ptr(state), ptr(last), ptr(cu_seqlens), B, S, H, HK, HD,
+                float(HD ** -0.5 if scale is None else scale), 1 if own else 0, ptr(ws), need), q, "a2v_linear_attention_fwd")
+    return out, last
+
+
+def linear_attention_bwd(q, k, v, slopes, d_out, *, scale=None, state=None, d_state=None, cu_seqlens=None, dq=None, dk=None, dv=None):
+    """-> dq, dk, dv and the gradient of `state` (None without one).  d_state: gradient of the state behind the last row, or None.
+    dq, dk, dv: all three (views of a packed gradient, for instance) or none; rows outside every sequence as in linear_attention_fwd.
+    Gradients of a shared k / v head are summed over its heads in fp32; nothing here depends on the order of arrival."""
+    B, S, H, HK, HD = _linear_attention_args("linear_attention_bwd", q, k, v, slopes, state, cu_seqlens)
+    _results("linear_attention_bwd", (("d_out", d_out, q),), out=False)
+    if d_state is not None:
+        _f32("linear_attention_bwd: d_state", d_state, (B, H, HD, HD), q)
+    given = [t is not None for t in (dq, dk, dv)]
+    if any(given) and not all(given):
+        raise ValueError("linear_attention_bwd: dq, dk and dv come together or not at all")
+    own = not any(given)
+    if own:
+        dq, dk, dv = (_E(*t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    else:
+        _results("linear_attention_bwd", (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)))
+        _apart("linear_attention_bwd", (dq, dk, dv), (q, k, v, d_out))
+    first = _E(B, H, HD, HD, dtype=torch.float32, device=q.device) if state is not None else None
+    if B == 0:
+        return dq, dk, dv, first
+    need = _L().a2v_linear_attention_workspace(dt(q), 1, cu_seqlens is not None, B, S, H, HK, HD)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _on_device(_L().a2v_linear_attention_bwd,
+               (dt(q), ptr(q), ptr(k), ptr(v), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), _strides(q, k, v, d_out, dq, dk, dv), ptr(slopes), ptr(state),
+                ptr(d_state), ptr(first), ptr(cu_seqlens), B, S, H, HK, HD, float(HD ** -0.5 if scale is None else scale), 1 if own else 0,
+                ptr(ws), need), q, "a2v_linear_attention_bwd")
+    return dq, dk, dv, first
+
+
+def linear_attention_step(q, k, v, slopes, state, *, slots=None, scale=None, out=None):
+    """One row of each of N streams: q (N,H,HD), k, v (N,HK,HD) -> out (N,H,HD); state (pool,H,HD,HD) fp32 is updated in place.
+    slots (N) int32 on the device: the pool entry of each row (default row n).  Rows that name the same entry are successive rows of
+    one stream, in order; an entry outside the pool touches no state and gives zeros (padding rows of a captured graph)."""
+    what = "linear_attention_step"
+    _heads(f"{what}: q", q, 3)
+    _heads(f"{what}: k", k, 3, q)
+    _heads(f"{what}: v", v, 3, q)
+    N, H, HD = q.shape
+    HK = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != N or k.shape[2] != HD or H < 1 or HK < 1 or H % HK:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    _f32(f"{what}: slopes", slopes, (H,), q)
+    _f32(f"{what}: state", state, (state.shape[0], H, HD, HD), q)
+    if slots is None:
+        if state.shape[0] < N:
+            raise ValueError(f"{what}: {N} rows and {state.shape[0]} states")
+    elif slots.dtype != torch.int32 or slots.device != q.device or tuple(slots.shape) != (N,) or not slots.is_contiguous():
+        raise ValueError(f"{what}: slots int32 ({N},) on {q.device} expected, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+    if out is None:
+        out = _E(N, H, HD, dtype=q.dtype, device=q.device)
+    else:
+        _results(what, (("out", out, q),))
+        _apart(what, (out,), (q, k, v))
+    if N == 0:
+        return out
+    st = (C.c_longlong * 8)(*[s if n > 1 else 0 for t in (q, k, v, out) for s, n in zip(t.stride()[:2], t.shape)])
+    _on_device(_L().a2v_linear_attention_step,
+               (dt(q), ptr(q), ptr(k), ptr(v), ptr(out), st, ptr(slopes), ptr(state), ptr(slots), state.shape[0], N, H, HK, HD,
+                float(HD ** -0.5 if scale is None else scale)), q, "a2v_linear_attention_step")
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
 #                                         normalisation
 # ----------------------------------------------------------------------------------------------
 def layernorm_fwd(x, gamma, beta, eps, *, res=None, act=0, save_stats=True, out=None, sum_out=None, post=None, drop=None):

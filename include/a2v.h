@@ -183,6 +183,54 @@ int a2v_attention_bwd(int dtype, const void* qkv, const void* out, const void* d
 int a2v_attention_bwd_fused_bias(int dtype, int S, int HD);
 int a2v_attention_bwd_direct_dq(int dtype, int S, int HD);
 
+/* ---------------------------------------------------------------- norm + rotation of q and k, linear attention
+ * For recordings and streams that are too long for a softmax over all frames: the scores are not normalised, the ALiBi term
+ * becomes a decay per head, and the whole past is one HD x HD state.  Nothing in the reference has this form; the calls stand
+ * where AltAttention.forward's q, k, v meet (modules.py:368-410) and take them as views of the qkv Linear's output.
+ *
+ * `strides` is a HOST array: (sequence, row, head) strides in elements, three per tensor in the order of the tensor arguments;
+ * the HD channels of a head are contiguous.  Pointers and strides are multiples of 16 bytes.  HD is 32, 64 or 128.  q and out have H
+ * heads, k and v HK (H % HK == 0: head h reads k / v head h / (H / HK)); gradients of a shared head are summed over its heads.
+ *
+ * a2v_qk_norm_rope: y = R(pos) (x r w), r = (mean x^2 + eps)^-1/2 over the channels of a head; q_weight / k_weight (HD) fp32.
+ * R turns `half` = sum(sections) channel pairs (a multiple of 8, <= HD / 2) -- (p, p + half), or (2p, 2p + 1) with `interleaved` -- by
+ * pos[axis of p] * inv_freq[p]; channels from 2 half on are only normalised.  sections: HOST array, pairs of each of the 1..3 axes.
+ * pos int32: element (n, s, axis) at n * pos_strides[0] + s * pos_strides[1] + axis; NULL = the row's index (one axis).
+ * q_out / k_out (backward: dq / dk) may be the inputs themselves (dq_out / dk_out), not otherwise overlap them.
+ * Backward: dq_weight / dk_weight are accumulated in a fixed order; ws: a2v_qk_norm_rope_workspace() bytes, 16-byte aligned. */
+int a2v_qk_norm_rope_fwd(int dtype, const void* q, const void* k, void* q_out, void* k_out, const long long* strides, const float* q_weight,
+                         const float* k_weight, const float* inv_freq, const int* pos, const long long* pos_strides, int axes,
+                         const int* sections, int interleaved, float eps, int N, int S, int H, int HK, int HD, a2v_stream_t stream);
+int a2v_qk_norm_rope_bwd(int dtype, const void* dq_out, const void* dk_out, const void* q, const void* k, void* dq, void* dk,
+                         const long long* strides, const float* q_weight, const float* k_weight, float* dq_weight /* += */,
+                         float* dk_weight /* += */, const float* inv_freq, const int* pos, const long long* pos_strides, int axes,
+                         const int* sections, int interleaved, float eps, int N, int S, int H, int HK, int HD, void* ws, size_t ws_bytes,
+                         a2v_stream_t stream);
+size_t a2v_qk_norm_rope_workspace(int N, int S, int H, int HK, int HD);
+/* S_t = exp(-slopes[h]) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t;  slopes (H) fp32, >= 0 (infinity: only the row itself).
+ * state / state_out (B, H, HD, HD) fp32 [channel of k][channel of v], before the first and behind the last row, either may be NULL;
+ * both may be the same buffer.
+ * cu_seqlens NULL: B sequences of S rows.  Else the tensors have S rows (sequence strides unused), sequence b is rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] (B + 1 int32 on the device, ascending; a sequence may be empty: its state is handed on).  Rows
+ * outside every sequence are left alone, or set to 0 with zero_outside.  Offsets outside [0, S] are clamped.
+ * ws: a2v_linear_attention_workspace() bytes (0 where the axis is not split), 16-byte aligned; used by this call only.
+ * dtype A2V_F32 or A2V_BF16; liba2v_hip_f16.so refuses its 16-bit type (A2V_ERR_UNSUPPORTED: a state does not fit half's range).
+ * A non-finite value reaches the rows of its own 64-row block and those behind it, never another sequence. */
+int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, const float* slopes,
+                             const float* state, float* state_out, const int* cu_seqlens, int B, int S, int H, int HK, int HD, float scale,
+                             int zero_outside, void* ws, size_t ws_bytes, a2v_stream_t stream);
+/* d_state_out: gradient of state_out or NULL; d_state: gradient of state or NULL.  No atomics: the same call gives the same bits. */
+int a2v_linear_attention_bwd(int dtype, const void* q, const void* k, const void* v, const void* d_out, void* dq, void* dk, void* dv,
+                             const long long* strides, const float* slopes, const float* state, const float* d_state_out, float* d_state,
+                             const int* cu_seqlens, int B, int S, int H, int HK, int HD, float scale, int zero_outside, void* ws,
+                             size_t ws_bytes, a2v_stream_t stream);
+size_t a2v_linear_attention_workspace(int dtype, int backward, int packed, int B, int S, int H, int HK, int HD);
+/* One row of each of N streams; state (n_slots, H, HD, HD) is updated in place.  slots (N) int32 or NULL (= row n).  Rows that name the
+ * same slot are successive rows of one stream, in order; a slot outside [0, n_slots) touches no state and gives a row of zeros.
+ * strides: HOST array, (row, head) of q, k, v, out, multiples of 4 elements; pointers aligned to 4 elements. */
+int a2v_linear_attention_step(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, const float* slopes,
+                              float* state, const int* slots, int n_slots, int N, int H, int HK, int HD, float scale, a2v_stream_t stream);
+
 /* ---------------------------------------------------------------- normalisation
  * y = act( LN(x [+ res]) * gamma + beta ), act 0 none / 1 GELU; optional sum_out = x + res;
  * optional mean/rstd (M) fp32 saved for backward.
@@ -424,7 +472,8 @@ int a2v_split_bf16(const float* x, void* out, long long M, int K, long long ldx,
 int a2v_maskinfo(const unsigned char* mask, int* ids_keep, int* ids_restore, int* rows_bad, int N, int T, int K,
                  a2v_stream_t stream);
 
-/* 14: a2v_attention_fwd takes `qk_norms` (one more pointer, after dropmask; NULL = the ABI-13 behaviour); + epilogue flag A2V_EPI_QKNORM of a2v_conv_gemm.
+/* 14 (later builds, no signature changed): + a2v_qk_norm_rope_fwd / _bwd / _workspace, a2v_linear_attention_fwd / _bwd / _workspace / _step.
+ * 14: a2v_attention_fwd takes `qk_norms` (one more pointer, after dropmask; NULL = the ABI-13 behaviour); + epilogue flag A2V_EPI_QKNORM of a2v_conv_gemm.
  * 13: a2v_attention_fwd / a2v_attention_bwd take `dropmask` (one more pointer each, after mdist; NULL = the ABI-12 arithmetic); + a2v_attention_dropmask_words;
  *     a2v_debug_set key 39 (round-6 whole-sequence attention kernels on / off).
  * 12: + a2v_conv_sparse_in, a2v_conv_wgrad_kept.
