@@ -28,6 +28,7 @@ struct LinRole {
   int qr, kr, vr;                                                // heads that share one head of the operand
   int reverse;                                                   // rows are visited from the last to the first
   int first_t;                                                   // `first` is read transposed
+  int ws_t;                                                      // so are the segment states: they are another role's
   int o32;                                                       // o is fp32 whatever the operands are
   float s_inter, s_state;                                        // factors of Y^T q and of k v^T (their product is the scale)
   const float* first;                                            // (B, H, HD, HD) state before the first row, or null
@@ -42,11 +43,12 @@ struct LinArgs {
   int seg;                                                       // rows of a segment, a multiple of the chunk
   int slots;                                                     // grid.x / H
   int fill;                                                      // rows outside every sequence become 0 (cu)
+  int roles, roles_state, split;                                 // roles of the main and of the state kernel; the axis is cut into segments
 };
 
 template <typename T> struct LinT;
 template <> struct LinT<bf16> {
-  static constexpr int C = 64, V = 8;                            // rows of a chunk, elements of a 16-byte load
+  static constexpr int C = 32, V = 8;                            // rows of a chunk, elements of a 16-byte load
   static constexpr bool SPLIT = true;
   typedef bf16x8 frag;
   static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, const f32x4& c) { return A2V_MFMA_16x16x32(a, b, c, 0, 0, 0); }
@@ -139,22 +141,28 @@ __device__ __forceinline__ float lin_log2(const float* slopes, int h) {
   const float l2 = -slopes[h] * 1.44269504088896341f;
   return l2 < -4096.f ? -4096.f : l2;                            // (an infinite slope: l^0 = 1, l^n = 0; NaN stays NaN)
 }
+__device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 template <typename T, int HD, bool STATE>
-__global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
+__global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT ? 3 : 4) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
   typedef typename L::frag frag;
   constexpr int C = L::C, NT = C / 16, NS = C / 32, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, P = lin_pitch<T, HD>();
-  constexpr int CPR = HD / L::V;                                 // 16-byte pieces of a row; C * CPR / THREADS = 2 for every T and HD
-  static_assert(C * CPR == 2 * THREADS, "two pieces per thread and tile");
-  __shared__ __attribute__((aligned(16))) T sm[3][C * P];
-  T* const sQ = sm[0];
-  T* const sK = sm[1];
-  T* const sV = sm[2];
-  const LinRole& r = a.r[blockIdx.y];
-  const int slot = blockIdx.x / a.H, h = blockIdx.x - slot * a.H;
+  constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
+  static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
+  __shared__ __attribute__((aligned(16))) T sm[STATE ? 2 : 4][C * P];
+  T* const sK = sm[0];
+  T* const sV = sm[1];
+  T* const sQ = sm[STATE ? 0 : 2];
+  T* const sO = sm[STATE ? 0 : 3];
+  // x = (slot, head, role): the roles of one (slot, head) read the same rows at the same time.  The main kernel of a split axis starts
+  // with the last segments: their k and v are what the state kernel has read last and the memory-side cache still holds.
+  const int nr = STATE ? a.roles_state : a.roles;
+  const int id = blockIdx.x / nr, slot0 = id / a.H, h = id - slot0 * a.H;
+  const LinRole& r = a.r[blockIdx.x - id * nr];
+  const int slot = !STATE && a.split ? a.slots - 1 - slot0 : slot0;
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, n0 = (tid >> 6) * 16;
   LinSeq s;
   const bool mine = lin_find(a, slot, s);
@@ -197,21 +205,27 @@ __global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
         }
     }
     if (s.p) {
-      const f32x4* const w = (const f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
+      const float* const w = r.ws + ((long long)slot * a.H + h) * HD * HD;
 #pragma unroll
-      for (int t = 0; t < ND; ++t) S[t] += w[t * 64];
+      for (int t = 0; t < ND; ++t) {
+        if (!r.ws_t) S[t] += *(const f32x4*)(w + (((tid >> 6) * ND + t) * 64 + lane) * 4);
+        else                                                     // element (16 t + 4 g + i, n0 + fr) of the transpose
+#pragma unroll
+          for (int i = 0; i < 4; ++i) S[t][i] += w[((t * ND + (tid >> 6)) * 64 + (fr >> 2) * 16 + 4 * g + i) * 4 + (fr & 3)];
+      }
     }
   }
 
   const T* const q = (const T*)r.q + (a.cu ? 0 : b * r.qn) + (long long)(h / r.qr) * r.qh;
   const T* const k = (const T*)r.k + (a.cu ? 0 : b * r.kn) + (long long)(h / r.kr) * r.kh;
   const T* const v = (const T*)r.v + (a.cu ? 0 : b * r.vn) + (long long)(h / r.vr) * r.vh;
+  T* const oB = oT + (a.cu ? 0 : b * r.on) + (long long)h * r.oh;
   const int row0 = r.reverse ? s.begin + s.len - 1 : s.begin, dir = r.reverse ? -1 : 1;      // row of position t: row0 + dir * t
 
-  uint4 pq[2], pk[2], pv[2];                                     // the next chunk's tiles, in flight during this one's math
+  uint4 pq[NU], pk[NU], pv[NU];                                     // the next chunk's tiles, in flight during this one's math
   auto fetch = [&](int t0) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < NU; ++u) {
       const int c = tid + u * THREADS, t = t0 + c / CPR, e = (c % CPR) * L::V;
       const uint4 z = {0u, 0u, 0u, 0u};
       pq[u] = z; pk[u] = z; pv[u] = z;
@@ -225,7 +239,7 @@ __global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
   };
   auto place = [&]() {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < NU; ++u) {
       const int c = tid + u * THREADS, at = (c / CPR) * P + (c % CPR) * L::V;
       if constexpr (!STATE) *(uint4*)(sQ + at) = pq[u];
       *(uint4*)(sK + at) = pk[u];
@@ -235,14 +249,15 @@ __global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
 
   // l^(i - j) scale for a query column fr and key rows 4 g + i: inside a tile, and one tile apart
   const float scale = r.s_inter * r.s_state;
-  float w0[4], w1[4];
+  float w0[4], w1[4], wv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int d = fr - 4 * g - i;
     w0[i] = d < 0 ? 0.f : scale * lin_pow(l2, d);
     w1[i] = scale * lin_pow(l2, 16 + d);
+    wv[i] = r.s_state * lin_pow(l2, 16 - 4 * g - i);
   }
-  const float l16 = lin_pow(l2, 16), lrow = r.s_inter * lin_pow(l2, fr);
+  const float l16 = lin_uniform(lin_pow(l2, 16)), l32 = lin_uniform(lin_pow(l2, 32)), l48 = lin_uniform(lin_pow(l2, 48)), lrow = r.s_inter * lin_pow(l2, fr);
 
   if (from < upto) fetch(from);
   for (int t0 = from; t0 < upto; t0 += C) {
@@ -255,70 +270,53 @@ __global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
 #pragma unroll
     for (int ks = 0; ks < NS; ++ks) vf[ks] = lin_col<T, HD>(sV, ks, n0, lane);
     if constexpr (!STATE) {
-      f32x4 acc[NT];
-      {
-        frag sh_[NK], sl_[NK];
+      frag yh[NK], yl[NK];
 #pragma unroll
-        for (int kd = 0; kd < NK; ++kd) {
-          float x[8];
+      for (int kd = 0; kd < NK; ++kd) {
+        float x[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
-          lin_split<T>(x, sh_[kd], sl_[kd]);
-        }
-        float f = lrow;
-#pragma unroll
-        for (int ti = 0; ti < NT; ++ti) {
-          acc[ti] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kd = 0; kd < NK; ++kd) {
-            const frag qf = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
-            acc[ti] = L::mma(sh_[kd], qf, acc[ti]);
-            if constexpr (L::SPLIT) acc[ti] = L::mma(sl_[kd], qf, acc[ti]);
-          }
-          acc[ti] *= f;
-          f *= l16;
-        }
+        for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
+        lin_split<T>(x, yh[kd], yl[kd]);
       }
+      float f = lrow;
 #pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {
-        frag ka[NK], kb[NK];
+      for (int ti = 0; ti < NT; ++ti) {                          // one tile of 16 query rows at a time (registers: see the launch bounds)
+        frag qf[NK];
+        f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kd = 0; kd < NK; ++kd) {
-          ka[kd] = lin_row<T, HD>(sK, 32 * ks + fr, kd, g);
-          kb[kd] = lin_row<T, HD>(sK, 32 * ks + 16 + fr, kd, g);
+          qf[kd] = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
+          acc = L::mma(yh[kd], qf[kd], acc);
+          if constexpr (L::SPLIT) acc = L::mma(yl[kd], qf[kd], acc);
         }
-        float fa = 1.f, fb = 1.f;                                // l^(16 (tiles between the query's and the key's, less one))
+        acc *= f;
+        f *= l16;
 #pragma unroll
-        for (int ti = 2 * ks; ti < NT; ++ti) {
-          f32x4 pa = (f32x4){0.f, 0.f, 0.f, 0.f}, pb = pa;
-#pragma unroll
-          for (int kd = 0; kd < NK; ++kd) {
-            const frag qf = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
-            pa = L::mma(ka[kd], qf, pa);
-            if (ti > 2 * ks) pb = L::mma(kb[kd], qf, pb);
-          }
+        for (int ks = 0; 2 * ks <= ti; ++ks) {
           float x[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // on the diagonal a select, not a product: a non-finite key does not reach the rows in front of it
-            x[i] = ti == 2 * ks ? (fr < 4 * g + i ? 0.f : pa[i] * w0[i]) : pa[i] * (w1[i] * fa);
-            x[4 + i] = ti == 2 * ks ? 0.f : ti == 2 * ks + 1 ? (fr < 4 * g + i ? 0.f : pb[i] * w0[i]) : pb[i] * (w1[i] * fb);
+          for (int e = 0; e < 2; ++e) {
+            const int d = ti - 2 * ks - e;                       // tiles between the queries and the keys
+            f32x4 p = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (d >= 0)
+#pragma unroll
+              for (int kd = 0; kd < NK; ++kd) p = L::mma(lin_row<T, HD>(sK, 32 * ks + 16 * e + fr, kd, g), qf[kd], p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              // on the diagonal a select, not a product: a non-finite key does not reach the rows in front of it
+              x[4 * e + i] = d < 0 ? 0.f : d == 0 ? (fr < 4 * g + i ? 0.f : p[i] * w0[i]) : (d == 1 ? p[i] : p[i] * (d == 2 ? l16 : l32)) * w1[i];
           }
           frag hi, lo;
           lin_split<T>(x, hi, lo);
-          acc[ti] = L::mma(vf[ks], hi, acc[ti]);
-          if constexpr (L::SPLIT) acc[ti] = L::mma(vf[ks], lo, acc[ti]);
-          if (ti > 2 * ks) { fb = fa; fa *= l16; }
+          acc = L::mma(vf[ks], hi, acc);
+          if constexpr (L::SPLIT) acc = L::mma(vf[ks], lo, acc);
         }
-      }
-#pragma unroll
-      for (int ti = 0; ti < NT; ++ti) {
-        const int t = t0 + 16 * ti + fr;
-        if (t < upto) {
-          const long long at = (a.cu ? 0 : b * r.on) + (long long)(row0 + dir * t) * r.os + (long long)h * r.oh + n0 + 4 * g;
-          if (r.o32) *(f32x4*)(oF + at) = acc[ti];
-          else Vec4<T>::store(oT + at, acc[ti]);
+        if (!r.o32) Vec4<T>::store(sO + (16 * ti + fr) * P + n0 + 4 * g, acc);
+        else {
+          const int t = t0 + 16 * ti + fr;
+          if (t < upto) *(f32x4*)(oF + (a.cu ? 0 : b * r.on) + (long long)(row0 + dir * t) * r.os + (long long)h * r.oh + n0 + 4 * g) = acc;
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     const bool last = ends && t0 + C >= upto;
@@ -330,22 +328,49 @@ __global__ __launch_bounds__(HD * 4) void lin_kernel(LinArgs a) {
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
         float x[8];
+        if (e == C) {                                            // l^(C - j), j = 16 tile + 4 g + i: a factor of the lane and one of the tile
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int n = e - (32 * ks + 16 * (i >> 2) + 4 * g + (i & 3));
-          x[i] = (float)vf[ks][i] * (r.s_state * lin_pow(l2, n < 0 ? 0 : n));        // rows behind the end hold 0
+          for (int i = 0; i < 8; ++i) {
+            const int up = NT - 1 - 2 * ks - (i >> 2);           // tiles behind this one
+            x[i] = ((float)vf[ks][i] * (up == 0 ? 1.f : up == 1 ? l16 : up == 2 ? l32 : l48)) * wv[i & 3];
+          }
+        } else {
+          int j0 = 4 * g;
+          asm volatile("" : "+v"(j0));                           // (keeps 16 lane constants of this rare branch out of the loop's registers)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int n = e - (32 * ks + 16 * (i >> 2) + (i & 3)) - j0;
+            x[i] = (float)vf[ks][i] * (r.s_state * lin_pow(l2, n < 0 ? 0 : n));      // rows behind the end hold 0
+          }
         }
-        frag hi, lo;
+        frag hi, lo, lo2;
         lin_split<T>(x, hi, lo);
+        if constexpr (L::SPLIT) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) lo2[i] = (T)(x[i] - (float)hi[i] - (float)lo[i]);
+        }
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
           const frag kf = lin_col<T, HD>(sK, ks, 16 * t, lane);
           S[t] = L::mma(kf, hi, S[t]);
-          if constexpr (L::SPLIT) S[t] = L::mma(kf, lo, S[t]);
+          if constexpr (L::SPLIT) {
+            S[t] = L::mma(kf, lo, S[t]);
+            S[t] = L::mma(kf, lo2, S[t]);
+          }
         }
       }
     }
     __syncthreads();
+    if constexpr (!STATE) {
+      // whole rows, 16 bytes a lane: 8-byte pieces straight from the accumulators cost 10 % of the launch
+      if (!r.o32) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const int at = tid + u * THREADS, t = t0 + at / CPR, el = (at % CPR) * L::V;
+          if (t < upto) *(uint4*)(oB + (row0 + dir * t) * r.os + el) = *(const uint4*)(sO + (at / CPR) * P + el);
+        }
+      }
+    }
   }
   if constexpr (STATE) {
     f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
@@ -497,7 +522,7 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
   if (rows >= (1LL << 30)) return false;
   p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
   const long long slots = packed ? (long long)S / p.seg + B + 1 : (long long)B * (S > p.seg ? (S + p.seg - 1) / p.seg : 1);
-  if (slots * H >= (1LL << 31)) return false;
+  if (slots * H * 3 >= (1LL << 31)) return false;
   p.slots = (int)slots;
   p.split = S > p.seg;
   p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
@@ -511,19 +536,20 @@ static bool lin_tensor_ok(const void* p, const long long* st, int es) {
 }
 
 template <typename T, int HD>
-static void lin_launch_hd(const LinArgs& a, const LinPlan& p, int roles, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.slots * (long long)a.H), roles), block(HD * 4);
+static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
+  const long long n = (long long)p.slots * a.H;
+  const dim3 block(HD * 4);
   if (p.split) {
-    hipLaunchKernelGGL((lin_kernel<T, HD, true>), grid, block, 0, stream, a);
-    hipLaunchKernelGGL(lin_scan_kernel, dim3(a.H * HD * HD / 1024, a.B, roles), dim3(256), 0, stream, a, HD * HD);
+    hipLaunchKernelGGL((lin_kernel<T, HD, true>), dim3((unsigned)(n * a.roles_state)), block, 0, stream, a);
+    hipLaunchKernelGGL(lin_scan_kernel, dim3(a.H * HD * HD / 1024, a.B, a.roles_state), dim3(256), 0, stream, a, HD * HD);
   }
-  hipLaunchKernelGGL((lin_kernel<T, HD, false>), grid, block, 0, stream, a);
+  hipLaunchKernelGGL((lin_kernel<T, HD, false>), dim3((unsigned)(n * a.roles)), block, 0, stream, a);
 }
 template <typename T>
-static void lin_launch(const LinArgs& a, const LinPlan& p, int roles, int HD, hipStream_t stream) {
-  if (HD == 32) lin_launch_hd<T, 32>(a, p, roles, stream);
-  else if (HD == 64) lin_launch_hd<T, 64>(a, p, roles, stream);
-  else lin_launch_hd<T, 128>(a, p, roles, stream);
+static void lin_launch(const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {
+  if (HD == 32) lin_launch_hd<T, 32>(a, p, stream);
+  else if (HD == 64) lin_launch_hd<T, 64>(a, p, stream);
+  else lin_launch_hd<T, 128>(a, p, stream);
 }
 static int lin_dtype(int dtype) {
   if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
@@ -537,7 +563,7 @@ extern "C" size_t a2v_linear_attention_workspace(int dtype, int backward, int pa
   LinPlan p;
   if (!lin_shape_ok(B, S, H, HK, HD) || !lin_plan(dtype, B, S, H, HD, packed != 0, p)) return 0;
   const size_t rows = packed ? (size_t)S : (size_t)B * S;
-  return (backward ? 3 : 1) * p.states + (backward && H != HK ? 2 * rows * H * HD * sizeof(float) : 0);
+  return (backward ? 2 : 1) * p.states + (backward && H != HK ? 2 * rows * H * HD * sizeof(float) : 0);
 }
 
 extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides,
@@ -555,10 +581,11 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
   a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
   LinRole& r = a.r[0];
   r = LinRole{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10],
-              strides[11], 1, H / HK, H / HK, 0, 0, 0, scale, 1.f, state, state_out, (float*)ws};
+              strides[11], 1, H / HK, H / HK, 0, 0, 0, 0, scale, 1.f, state, state_out, (float*)ws};
   a.r[1] = a.r[2] = r;
-  if (dtype == A2V_F32) lin_launch<float>(a, p, 1, HD, stream);
-  else lin_launch<bf16>(a, p, 1, HD, stream);
+  a.roles = a.roles_state = 1; a.split = p.split;
+  if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
+  else lin_launch<bf16>(a, p, HD, stream);
   A2V_CHECK_LAUNCH();
   return A2V_OK;
 }
@@ -580,25 +607,26 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
   if (need > ws_bytes || (need && (!ws || ((uintptr_t)ws & 15)))) return A2V_ERR_ARG;
   char* w = (char*)ws;
   const size_t rows = cu_seqlens ? (size_t)S : (size_t)B * S;
-  float* const dk32 = (float*)(w + 3 * p.states);
+  float* const dk32 = (float*)(w + 2 * p.states);
   float* const dv32 = dk32 + rows * H * HD;
   const long long* const s = strides;
   const long long pn = (long long)S * H * HD, ps = (long long)H * HD;
   LinArgs a;
   a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
   a.r[0] = LinRole{d_out, v, k, dq, s[9], s[10], s[11], s[6], s[7], s[8], s[3], s[4], s[5], s[12], s[13], s[14],
-                   1, rep, rep, 0, 1, 0, scale, 1.f, state, nullptr, (float*)w};
+                   1, rep, rep, 0, 1, 0, 0, scale, 1.f, state, nullptr, (float*)w};
+  a.roles = 3; a.roles_state = 2; a.split = p.split;               // dk's segment states are the transposes of dv's
   a.r[1] = LinRole{k, q, d_out, dv, s[3], s[4], s[5], s[0], s[1], s[2], s[9], s[10], s[11], s[18], s[19], s[20],
-                   rep, 1, 1, 1, 0, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
+                   rep, 1, 1, 1, 0, 0, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
   a.r[2] = LinRole{v, d_out, q, dk, s[6], s[7], s[8], s[9], s[10], s[11], s[0], s[1], s[2], s[15], s[16], s[17],
-                   rep, 1, 1, 1, 1, 0, 1.f, scale, d_state_out, nullptr, (float*)(w + 2 * p.states)};
+                   rep, 1, 1, 1, 1, 1, 0, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
   if (rep > 1) {
     LinRole* const g[2] = {&a.r[1], &a.r[2]};
     float* const to[2] = {dv32, dk32};
     for (int i = 0; i < 2; ++i) { g[i]->o = to[i]; g[i]->on = pn; g[i]->os = ps; g[i]->oh = HD; g[i]->o32 = 1; }
   }
-  if (dtype == A2V_F32) lin_launch<float>(a, p, 3, HD, stream);
-  else lin_launch<bf16>(a, p, 3, HD, stream);
+  if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
+  else lin_launch<bf16>(a, p, HD, stream);
   if (rep > 1 && rows) {
     const dim3 grid((unsigned)cdiv((long)(rows * HK * HD / 4), 256));
     if (dtype == A2V_F32)
