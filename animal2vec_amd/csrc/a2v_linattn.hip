@@ -22,6 +22,8 @@
 
 typedef __attribute__((address_space(3))) s16x4 la_lds_s16x4;
 
+typedef __attribute__((ext_vector_type(4))) unsigned lin_raw;     // 16 bytes in flight
+
 struct LinRole {
   const void* q; const void* k; const void* v; void* o;
   long long qn, qs, qh, kn, ks, kh, vn, vs, vh, on, os, oh;     // strides in elements: sequence, row, head
@@ -29,6 +31,7 @@ struct LinRole {
   int reverse;                                                   // rows are visited from the last to the first
   int first_t;                                                   // `first` is read transposed
   int ws_t;                                                      // so are the segment states: they are another role's
+  int exact;                                                     // 16-bit operands: the state keeps all of its 32 bits
   int o32;                                                       // o is fp32 whatever the operands are
   float s_inter, s_state;                                        // factors of Y^T q and of k v^T (their product is the scale)
   const float* first;                                            // (B, H, HD, HD) state before the first row, or null
@@ -102,11 +105,38 @@ template <typename T, int HD> __device__ __forceinline__ typename LinT<T>::frag 
   }
   return f;
 }
-template <typename T> __device__ __forceinline__ void lin_split(const float* x, typename LinT<T>::frag& hi, typename LinT<T>::frag& lo) {
+// x = hi + lo (+ lo2): the nearest 16-bit value, the nearest to what is left, and so on; two elements at a time (v_cvt_pk, then a shift
+// and a mask to get the pair back: 6 instructions a pair and part)
+template <typename T, int PARTS> __device__ __forceinline__ void lin_split(const float* x, typename LinT<T>::frag* f) {
+  if constexpr (LinT<T>::SPLIT) {
+    union { unsigned w[4]; bf16x8 v; } u[PARTS];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi[i] = (T)x[i];
-    if constexpr (LinT<T>::SPLIT) lo[i] = (T)(x[i] - (float)hi[i]);
+    for (int i = 0; i < 4; ++i) {
+      float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) {
+        const bf16x2 h = __builtin_convertvector((f32x2){a, b}, bf16x2);
+        u[k].w[i] = __builtin_bit_cast(unsigned, h);
+        if (k + 1 < PARTS) { a -= a2v_lo16_f32(u[k].w[i]); b -= a2v_hi16_f32(u[k].w[i]); }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) f[k] = u[k].v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[0][i] = x[i];
+  }
+}
+
+// S += k^T x over 32 rows of the tile, x (the wave's 16 columns, weighted) in PARTS 16-bit parts
+template <typename T, int HD, int PARTS> __device__ __forceinline__ void lin_update(f32x4* S, const float* x, const T* sK, int ks, int lane) {
+  typename LinT<T>::frag p[PARTS];
+  lin_split<T, PARTS>(x, p);
+#pragma unroll
+  for (int t = 0; t < HD / 16; ++t) {
+    const typename LinT<T>::frag kf = lin_col<T, HD>(sK, ks, 16 * t, lane);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) S[t] = LinT<T>::mma(kf, p[i], S[t]);
   }
 }
 
@@ -146,7 +176,7 @@ __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amd
 
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 template <typename T, int HD, bool STATE>
-__global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT ? 3 : 4) void lin_kernel(LinArgs a) {
+__global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
   typedef typename L::frag frag;
   constexpr int C = L::C, NT = C / 16, NS = C / 32, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, P = lin_pitch<T, HD>();
@@ -222,28 +252,44 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT
   T* const oB = oT + (a.cu ? 0 : b * r.on) + (long long)h * r.oh;
   const int row0 = r.reverse ? s.begin + s.len - 1 : s.begin, dir = r.reverse ? -1 : 1;      // row of position t: row0 + dir * t
 
-  uint4 pq[NU], pk[NU], pv[NU];                                     // the next chunk's tiles, in flight during this one's math
-  auto fetch = [&](int t0) {
+  // A tile's rows t0 .. t0 + c - 1 lie at row `low` and above, in reverse order backwards: a uniform address and an offset per piece that
+  // only the last chunk changes.  Its missing rows are copies of the last one (whatever they hold meets a zero weight).
+  lin_raw pq[NU], pk[NU], pv[NU];                                 // the next chunk's tiles, in flight during this one's math
+  unsigned aq[NU], ak[NU], av[NU], ao[NU];
+  auto offsets = [&](unsigned (&off)[NU], long long stride, int c) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int c = tid + u * THREADS, t = t0 + c / CPR, e = (c % CPR) * L::V;
-      const uint4 z = {0u, 0u, 0u, 0u};
-      pq[u] = z; pk[u] = z; pv[u] = z;
-      if (t < upto) {
-        const long long row = row0 + dir * t;
-        if constexpr (!STATE) pq[u] = *(const uint4*)(q + row * r.qs + e);
-        pk[u] = *(const uint4*)(k + row * r.ks + e);
-        pv[u] = *(const uint4*)(v + row * r.vs + e);
-      }
+      const int at = tid + u * THREADS, i = at / CPR < c ? at / CPR : c - 1;
+      off[u] = (unsigned)(r.reverse ? c - 1 - i : i) * (unsigned)(stride * sizeof(T)) + (at % CPR) * 16;
     }
   };
-  auto place = [&]() {
+  auto offsets_in = [&](int c) __attribute__((always_inline)) {
+    if constexpr (!STATE) offsets(aq, r.qs, c);
+    offsets(ak, r.ks, c);
+    offsets(av, r.vs, c);
+  };
+  auto low = [&](int t0, int c) { return (long long)(r.reverse ? row0 - t0 - (c - 1) : row0 + t0); };
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+    const int c = upto - t0 < C ? upto - t0 : C;
+    const long long n = low(t0, c);
+    const char* const bq = (const char*)(q + n * r.qs);
+    const char* const bk = (const char*)(k + n * r.ks);
+    const char* const bv = (const char*)(v + n * r.vs);
+    if (c < C) offsets_in(c);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if constexpr (!STATE) pq[u] = *(const lin_raw*)(bq + aq[u]);
+      pk[u] = *(const lin_raw*)(bk + ak[u]);
+      pv[u] = *(const lin_raw*)(bv + av[u]);
+    }
+  };
+  auto place = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int c = tid + u * THREADS, at = (c / CPR) * P + (c % CPR) * L::V;
-      if constexpr (!STATE) *(uint4*)(sQ + at) = pq[u];
-      *(uint4*)(sK + at) = pk[u];
-      *(uint4*)(sV + at) = pv[u];
+      if constexpr (!STATE) *(lin_raw*)(sQ + at) = pq[u];
+      *(lin_raw*)(sK + at) = pk[u];
+      *(lin_raw*)(sV + at) = pv[u];
     }
   };
 
@@ -259,6 +305,8 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT
   }
   const float l16 = lin_uniform(lin_pow(l2, 16)), l32 = lin_uniform(lin_pow(l2, 32)), l48 = lin_uniform(lin_pow(l2, 48)), lrow = r.s_inter * lin_pow(l2, fr);
 
+  offsets_in(C);
+  if constexpr (!STATE) offsets(ao, r.os, C);
   if (from < upto) fetch(from);
   for (int t0 = from; t0 < upto; t0 += C) {
     const int c = upto - t0 < C ? upto - t0 : C;
@@ -270,13 +318,13 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT
 #pragma unroll
     for (int ks = 0; ks < NS; ++ks) vf[ks] = lin_col<T, HD>(sV, ks, n0, lane);
     if constexpr (!STATE) {
-      frag yh[NK], yl[NK];
+      frag y[NK][L::SPLIT ? 2 : 1];
 #pragma unroll
       for (int kd = 0; kd < NK; ++kd) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
-        lin_split<T>(x, yh[kd], yl[kd]);
+        lin_split<T, L::SPLIT ? 2 : 1>(x, y[kd]);
       }
       float f = lrow;
 #pragma unroll
@@ -286,8 +334,8 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT
 #pragma unroll
         for (int kd = 0; kd < NK; ++kd) {
           qf[kd] = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
-          acc = L::mma(yh[kd], qf[kd], acc);
-          if constexpr (L::SPLIT) acc = L::mma(yl[kd], qf[kd], acc);
+          acc = L::mma(y[kd][0], qf[kd], acc);
+          if constexpr (L::SPLIT) acc = L::mma(y[kd][1], qf[kd], acc);
         }
         acc *= f;
         f *= l16;
@@ -306,10 +354,10 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT
               // on the diagonal a select, not a product: a non-finite key does not reach the rows in front of it
               x[4 * e + i] = d < 0 ? 0.f : d == 0 ? (fr < 4 * g + i ? 0.f : p[i] * w0[i]) : (d == 1 ? p[i] : p[i] * (d == 2 ? l16 : l32)) * w1[i];
           }
-          frag hi, lo;
-          lin_split<T>(x, hi, lo);
-          acc = L::mma(vf[ks], hi, acc);
-          if constexpr (L::SPLIT) acc = L::mma(vf[ks], lo, acc);
+          frag p[L::SPLIT ? 2 : 1];
+          lin_split<T, L::SPLIT ? 2 : 1>(x, p);
+          acc = L::mma(vf[ks], p[0], acc);
+          if constexpr (L::SPLIT) acc = L::mma(vf[ks], p[1], acc);
         }
         if (!r.o32) Vec4<T>::store(sO + (16 * ti + fr) * P + n0 + 4 * g, acc);
         else {
@@ -339,35 +387,25 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : HD == 64 && !LinT<T>::SPLIT
           asm volatile("" : "+v"(j0));                           // (keeps 16 lane constants of this rare branch out of the loop's registers)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int n = e - (32 * ks + 16 * (i >> 2) + (i & 3)) - j0;
-            x[i] = (float)vf[ks][i] * (r.s_state * lin_pow(l2, n < 0 ? 0 : n));      // rows behind the end hold 0
+            const int j = j0 + 32 * ks + 16 * (i >> 2) + (i & 3);
+            x[i] = j < c ? (float)vf[ks][i] * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
           }
         }
-        frag hi, lo, lo2;
-        lin_split<T>(x, hi, lo);
-        if constexpr (L::SPLIT) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) lo2[i] = (T)(x[i] - (float)hi[i] - (float)lo[i]);
-        }
-#pragma unroll
-        for (int t = 0; t < ND; ++t) {
-          const frag kf = lin_col<T, HD>(sK, ks, 16 * t, lane);
-          S[t] = L::mma(kf, hi, S[t]);
-          if constexpr (L::SPLIT) {
-            S[t] = L::mma(kf, lo, S[t]);
-            S[t] = L::mma(kf, lo2, S[t]);
-          }
-        }
+        // a state that leaves the call (or might: out does not depend on that) keeps its 32 bits, three parts of 8; else two do
+        if (L::SPLIT && r.exact) lin_update<T, HD, L::SPLIT ? 3 : 1>(S, x, sK, ks, lane);
+        else lin_update<T, HD, L::SPLIT ? 2 : 1>(S, x, sK, ks, lane);
       }
     }
     __syncthreads();
     if constexpr (!STATE) {
       // whole rows, 16 bytes a lane: 8-byte pieces straight from the accumulators cost 10 % of the launch
       if (!r.o32) {
+        char* const bo = (char*)(oB + low(t0, c) * r.os);
+        if (c < C) offsets(ao, r.os, c);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-          const int at = tid + u * THREADS, t = t0 + at / CPR, el = (at % CPR) * L::V;
-          if (t < upto) *(uint4*)(oB + (row0 + dir * t) * r.os + el) = *(const uint4*)(sO + (at / CPR) * P + el);
+          const int at = tid + u * THREADS;
+          if (at / CPR < c) *(lin_raw*)(bo + ao[u]) = *(const lin_raw*)(sO + (at / CPR) * P + (at % CPR) * L::V);
         }
       }
     }
@@ -532,7 +570,8 @@ static bool lin_shape_ok(int B, int S, int H, int HK, int HD) {
   return B >= 0 && S >= 0 && H > 0 && HK > 0 && H % HK == 0 && H <= 65535 && B <= 65535 * 16 && (HD == 32 || HD == 64 || HD == 128);
 }
 static bool lin_tensor_ok(const void* p, const long long* st, int es) {
-  return p && !((uintptr_t)p & 15) && !((st[0] * es) & 15) && !((st[1] * es) & 15) && !((st[2] * es) & 15);
+  return p && !((uintptr_t)p & 15) && !((st[0] * es) & 15) && !((st[1] * es) & 15) && !((st[2] * es) & 15) && st[1] >= 0 &&
+         st[1] * es < (1 << 26);                                 // (offsets inside a chunk are 32 bits)
 }
 
 template <typename T, int HD>
@@ -581,7 +620,7 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
   a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
   LinRole& r = a.r[0];
   r = LinRole{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10],
-              strides[11], 1, H / HK, H / HK, 0, 0, 0, 0, scale, 1.f, state, state_out, (float*)ws};
+              strides[11], 1, H / HK, H / HK, 0, 0, 0, 1, 0, scale, 1.f, state, state_out, (float*)ws};
   a.r[1] = a.r[2] = r;
   a.roles = a.roles_state = 1; a.split = p.split;
   if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
@@ -614,12 +653,12 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
   LinArgs a;
   a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
   a.r[0] = LinRole{d_out, v, k, dq, s[9], s[10], s[11], s[6], s[7], s[8], s[3], s[4], s[5], s[12], s[13], s[14],
-                   1, rep, rep, 0, 1, 0, 0, scale, 1.f, state, nullptr, (float*)w};
+                   1, rep, rep, 0, 1, 0, 0, 0, scale, 1.f, state, nullptr, (float*)w};
   a.roles = 3; a.roles_state = 2; a.split = p.split;               // dk's segment states are the transposes of dv's
   a.r[1] = LinRole{k, q, d_out, dv, s[3], s[4], s[5], s[0], s[1], s[2], s[9], s[10], s[11], s[18], s[19], s[20],
-                   rep, 1, 1, 1, 0, 0, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
+                   rep, 1, 1, 1, 0, 0, d_state != nullptr, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
   a.r[2] = LinRole{v, d_out, q, dk, s[6], s[7], s[8], s[9], s[10], s[11], s[0], s[1], s[2], s[15], s[16], s[17],
-                   rep, 1, 1, 1, 1, 1, 0, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
+                   rep, 1, 1, 1, 1, 1, 0, 0, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
   if (rep > 1) {
     LinRole* const g[2] = {&a.r[1], &a.r[2]};
     float* const to[2] = {dv32, dk32};
