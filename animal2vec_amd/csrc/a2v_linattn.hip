@@ -44,8 +44,9 @@ struct LinArgs {
   const int* cu;                                                 // (B + 1) row offsets, or null: B sequences of S rows
   int B, S, H, T;                                                // T: rows in all (cu), S: rows of a sequence
   int seg;                                                       // rows of a segment, a multiple of the chunk
-  int slots;                                                     // grid.x / H
+  int slots;
   int fill;                                                      // rows outside every sequence become 0 (cu)
+  int rep;                                                       // heads that share one head of k and v
   int roles, roles_state, split;                                 // roles of the main and of the state kernel; the axis is cut into segments
 };
 
@@ -187,11 +188,14 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
   T* const sV = sm[1];
   T* const sQ = sm[STATE ? 0 : 2];
   T* const sO = sm[STATE ? 0 : 3];
-  // x = (slot, head, role): the roles of one (slot, head) read the same rows at the same time.  The main kernel of a split axis starts
-  // with the last segments: their k and v are what the state kernel has read last and the memory-side cache still holds.
-  const int nr = STATE ? a.roles_state : a.roles;
-  const int id = blockIdx.x / nr, slot0 = id / a.H, h = id - slot0 * a.H;
-  const LinRole& r = a.r[blockIdx.x - id * nr];
+  // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
+  // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
+  const int nr = STATE ? a.roles_state : a.roles, nin = nr * a.rep, HK = a.H / a.rep;
+  const int grp = blockIdx.x / (8 * nin), rem = blockIdx.x - grp * 8 * nin, in = rem >> 3, unit = grp * 8 + (rem & 7);
+  const int slot0 = unit / HK, h = (unit - slot0 * HK) * a.rep + in / nr;
+  if (slot0 >= a.slots) return;
+  const LinRole& r = a.r[in % nr];
+  // the main kernel of a split axis starts with the last segments: their k and v are what the state kernel has read last
   const int slot = !STATE && a.split ? a.slots - 1 - slot0 : slot0;
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, n0 = (tid >> 6) * 16;
   LinSeq s;
@@ -364,7 +368,6 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
           const int t = t0 + 16 * ti + fr;
           if (t < upto) *(f32x4*)(oF + (a.cu ? 0 : b * r.on) + (long long)(row0 + dir * t) * r.os + (long long)h * r.oh + n0 + 4 * g) = acc;
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
     }
     const bool last = ends && t0 + C >= upto;
@@ -398,14 +401,15 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
     }
     __syncthreads();
     if constexpr (!STATE) {
-      // whole rows, 16 bytes a lane: 8-byte pieces straight from the accumulators cost 10 % of the launch
+      // whole rows, 16 bytes a lane: 8-byte pieces straight from the accumulators cost 10 % of the launch.  Past the L2, which the
+      // operands need: 2 to 5 % on every long case.
       if (!r.o32) {
         char* const bo = (char*)(oB + low(t0, c) * r.os);
         if (c < C) offsets(ao, r.os, c);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           const int at = tid + u * THREADS;
-          if (at / CPR < c) *(lin_raw*)(bo + ao[u]) = *(const lin_raw*)(sO + (at / CPR) * P + (at % CPR) * L::V);
+          if (at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (at / CPR) * P + (at % CPR) * L::V), (lin_raw*)(bo + ao[u]));
         }
       }
     }
@@ -560,7 +564,7 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
   if (rows >= (1LL << 30)) return false;
   p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
   const long long slots = packed ? (long long)S / p.seg + B + 1 : (long long)B * (S > p.seg ? (S + p.seg - 1) / p.seg : 1);
-  if (slots * H * 3 >= (1LL << 31)) return false;
+  if ((slots + 8) * H * 3 >= (1LL << 31)) return false;
   p.slots = (int)slots;
   p.split = S > p.seg;
   p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
@@ -576,7 +580,7 @@ static bool lin_tensor_ok(const void* p, const long long* st, int es) {
 
 template <typename T, int HD>
 static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
-  const long long n = (long long)p.slots * a.H;
+  const long long n = ((long long)p.slots * (a.H / a.rep) + 7) / 8 * 8 * a.rep;
   const dim3 block(HD * 4);
   if (p.split) {
     hipLaunchKernelGGL((lin_kernel<T, HD, true>), dim3((unsigned)(n * a.roles_state)), block, 0, stream, a);
@@ -622,7 +626,7 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
   r = LinRole{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10],
               strides[11], 1, H / HK, H / HK, 0, 0, 0, 1, 0, scale, 1.f, state, state_out, (float*)ws};
   a.r[1] = a.r[2] = r;
-  a.roles = a.roles_state = 1; a.split = p.split;
+  a.roles = a.roles_state = 1; a.split = p.split; a.rep = H / HK;
   if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
   else lin_launch<bf16>(a, p, HD, stream);
   A2V_CHECK_LAUNCH();
@@ -654,7 +658,7 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
   a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
   a.r[0] = LinRole{d_out, v, k, dq, s[9], s[10], s[11], s[6], s[7], s[8], s[3], s[4], s[5], s[12], s[13], s[14],
                    1, rep, rep, 0, 1, 0, 0, 0, scale, 1.f, state, nullptr, (float*)w};
-  a.roles = 3; a.roles_state = 2; a.split = p.split;               // dk's segment states are the transposes of dv's
+  a.roles = 3; a.roles_state = 2; a.split = p.split; a.rep = rep;               // dk's segment states are the transposes of dv's
   a.r[1] = LinRole{k, q, d_out, dv, s[3], s[4], s[5], s[0], s[1], s[2], s[9], s[10], s[11], s[18], s[19], s[20],
                    rep, 1, 1, 1, 0, 0, d_state != nullptr, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
   a.r[2] = LinRole{v, d_out, q, dk, s[6], s[7], s[8], s[9], s[10], s[11], s[0], s[1], s[2], s[15], s[16], s[17],

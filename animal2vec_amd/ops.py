@@ -565,13 +565,45 @@ def rope_inv_freq(sections, base=10000.0, device="cuda"):
     return torch.cat([base ** (-torch.arange(n, dtype=torch.float64) / max(1, n)) for n in sections]).float().to(device)
 
 
-def _on_device(fn, args, t, what):
-    """fn(*args, stream) on the current stream of t's device, which need not be the current device"""
-    if t.device.index == torch.cuda.current_device():
-        check(fn(*args, stream()), what)
+# A call's checks, strides and sizes depend on layouts alone (shapes, strides, types, devices, options): they are worked out once per
+# layout, so that the next frame of a stream pays for a dictionary look-up.  Nothing of the tensors themselves is kept; what depends on
+# addresses (alignment, overlap) is checked in every call.
+_LAYOUTS = {}
+
+
+def _layout(name, opts, ts, make):
+    key = (name, _HALF, opts, *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in ts])
+    p = _LAYOUTS.get(key)
+    if p is None:
+        p = make()
+        if len(_LAYOUTS) >= 1024:
+            _LAYOUTS.clear()
+        _LAYOUTS[key] = p
+    return p
+
+
+def _run(fn, what, device, *args):
+    """fn(*args, stream) on the current stream of `device`, which need not be the current device"""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device.index))
     else:
-        with torch.cuda.device(t.device):
-            check(fn(*args, stream()), what)
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device.index))
+    if rc:
+        check(rc, what)
+
+
+# the handle without a Stream object around it, where this torch has it (1 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _starts(what, *ts):
+    """data pointers, on 16 bytes each"""
+    ps = [t.data_ptr() for t in ts]
+    for p in ps:
+        if p & 15:
+            raise ValueError(f"{what}: every tensor of heads must start on 16 bytes")
+    return ps
 
 
 def _heads(what, t, dims, like=None, out=False):
@@ -586,8 +618,10 @@ def _heads(what, t, dims, like=None, out=False):
     if t.numel() == 0:
         return
     st, per = t.stride(), per16(t)
-    if st[-1] != 1 or any(s % per for s, n in zip(st[:-1], t.shape) if n > 1) or t.data_ptr() % 16:
+    if st[-1] != 1 or any(s % per for s, n in zip(st[:-1], t.shape) if n > 1):
         raise ValueError(f"{what}: the channels of a head must be contiguous and every head start on 16 bytes, got strides {st}")
+    if dims == 4 and t.shape[1] > 1 and st[1] * t.element_size() >= 1 << 26:
+        raise ValueError(f"{what}: rows {st[1]} elements apart (most: 64 MiB)")
     if out and any(s < t.shape[-1] for s, n in zip(st[:-1], t.shape) if n > 1):
         raise ValueError(f"{what}: an output may not repeat memory, got strides {st}")
 
@@ -602,6 +636,11 @@ def _results(what, named, out=True):
 def _f32(what, t, shape, like):
     if t.dtype != torch.float32 or t.device != like.device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous float32 {tuple(shape)} on {like.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _on_gpu(t):
+    if not t.is_cuda:
+        raise _lib.A2VError("a2v ops need device tensors (no CPU path exists)")
 
 
 def _overlap(a, b):
@@ -639,7 +678,13 @@ def _strides(*ts):
     return (C.c_longlong * (3 * len(ts)))(*[s if n > 1 else 0 for t in ts for s, n in zip(t.stride()[:3], t.shape)])
 
 
-def _qk_norm_rope_args(what, q, k, q_weight, k_weight, inv_freq, pos, sections):
+def _like(t):
+    """a contiguous tensor of t's layout, at capacity inside an engine step (set_row_cap)"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format) if _ROWCAP is None else _E(*t.shape, dtype=t.dtype, device=t.device)
+
+
+def _qk_norm_rope_checks(what, q, k, q_weight, k_weight, inv_freq, pos, sections):
+    """-> code, position strides, axes, sections, sizes as the C entries take them"""
     _heads(f"{what}: q", q, 4)
     _heads(f"{what}: k", k, 4, q)
     N, S, H, HD = q.shape
@@ -661,7 +706,7 @@ def _qk_norm_rope_args(what, q, k, q_weight, k_weight, inv_freq, pos, sections):
         if pos.dtype != torch.int32 or pos.device != q.device or tuple(pos.shape) != want or (pos.dim() == 3 and pos.shape[2] > 1 and pos.stride(2) != 1):
             raise ValueError(f"{what}: pos int32 {want} on {q.device} expected, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
         ps = (C.c_longlong * 2)(*pos.stride()[:2])
-    return inv_freq, pos, ps, len(sections), (C.c_int * len(sections))(*sections)
+    return dt(q), ps, len(sections), (C.c_int * len(sections))(*sections), (N, S, H, k.shape[2], HD)
 
 
 def qk_norm_rope_fwd(q, k, q_weight, k_weight, inv_freq, pos=None, *, sections=None, interleaved=False, eps=1e-6, q_out=None, k_out=None):
@@ -672,21 +717,28 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, inv_freq, pos=None, *, sections=N
     (p, p + half), or (2p, 2p + 1) with interleaved=True; half is a multiple of 8 and at most HD / 2, the channels from 2 half on are
     only normalised.  sections: pairs per axis of the position (one to three axes: time, microphone, band ...), default one axis.
     pos int32 (N,S) or (N,S,axes), any sign, exact to 32 bits; None: the row's index."""
-    args = _qk_norm_rope_args("qk_norm_rope_fwd", q, k, q_weight, k_weight, inv_freq, pos, sections)
-    N, S, H, HD = q.shape
+    what = "qk_norm_rope_fwd"
     given = q_out is not None or k_out is not None
     if q_out is None:
-        q_out = _E(N, S, H, HD, dtype=q.dtype, device=q.device)
+        q_out = _like(q)
     if k_out is None:
-        k_out = _E(N, S, k.shape[2], HD, dtype=q.dtype, device=q.device)
+        k_out = _like(k)
+
+    def plan():
+        p = _qk_norm_rope_checks(what, q, k, q_weight, k_weight, inv_freq, pos, sections)
+        _results(what, (("q_out", q_out, q), ("k_out", k_out, k)))
+        if given:
+            _apart(what, (q_out, k_out), (q, k), (q, k))         # (before the device check: a refusal does not depend on the device)
+        _starts(what, q, k, q_out, k_out, q_weight, k_weight)
+        _on_gpu(q)
+        return (_strides(q, k, q_out, k_out), *p)
+    st, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections), (q, k, q_weight, k_weight, inv_freq, pos, *((q_out, k_out) if given else ())), plan)
     if given:
-        _results("qk_norm_rope_fwd", (("q_out", q_out, q), ("k_out", k_out, k)))
-        _apart("qk_norm_rope_fwd", (q_out, k_out), (q, k), (q, k))
+        _apart(what, (q_out, k_out), (q, k), (q, k))
     if q.numel() == 0:
         return q_out, k_out
-    _on_device(_L().a2v_qk_norm_rope_fwd,
-               (dt(q), ptr(q), ptr(k), ptr(q_out), ptr(k_out), _strides(q, k, q_out, k_out), ptr(q_weight), ptr(k_weight), ptr(args[0]), ptr(args[1]),
-                *args[2:], 1 if interleaved else 0, float(eps), N, S, H, k.shape[2], HD), q, "a2v_qk_norm_rope_fwd")
+    _run(_L().a2v_qk_norm_rope_fwd, "a2v_qk_norm_rope_fwd", q.device, code, *_starts(what, q, k, q_out, k_out), st, *_starts(what, q_weight, k_weight),
+         inv_freq.data_ptr(), None if pos is None else pos.data_ptr(), ps, axes, sec, 1 if interleaved else 0, eps, *sizes)
     return q_out, k_out
 
 
@@ -694,33 +746,41 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, inv_freq, pos=Non
                      eps=1e-6, dq=None, dk=None):
     """-> dq, dk, from the gradients of qk_norm_rope_fwd's results and its inputs (q and k as they were before an in-place call).
     dq_weight, dk_weight (HD) fp32 are accumulated, in the same order every time.  dq / dk may be dq_out / dk_out themselves."""
-    args = _qk_norm_rope_args("qk_norm_rope_bwd", q, k, q_weight, k_weight, inv_freq, pos, sections)
-    N, S, H, HD = q.shape
-    HK = k.shape[2]
-    _results("qk_norm_rope_bwd", (("dq_out", dq_out, q), ("dk_out", dk_out, k)), out=False)
+    what = "qk_norm_rope_bwd"
     given = dq is not None or dk is not None
     if dq is None:
-        dq = _E(N, S, H, HD, dtype=q.dtype, device=q.device)
+        dq = _like(q)
     if dk is None:
-        dk = _E(N, S, HK, HD, dtype=q.dtype, device=q.device)
-    _f32("qk_norm_rope_bwd: dq_weight", dq_weight, (HD,), q)
-    _f32("qk_norm_rope_bwd: dk_weight", dk_weight, (HD,), q)
+        dk = _like(k)
+
+    def plan():
+        p = _qk_norm_rope_checks(what, q, k, q_weight, k_weight, inv_freq, pos, sections)
+        _results(what, (("dq_out", dq_out, q), ("dk_out", dk_out, k)), out=False)
+        _results(what, (("dq", dq, q), ("dk", dk, k)))
+        _f32(f"{what}: dq_weight", dq_weight, (q.shape[3],), q)
+        _f32(f"{what}: dk_weight", dk_weight, (q.shape[3],), q)
+        if dq_weight.data_ptr() == dk_weight.data_ptr():
+            raise ValueError(f"{what}: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
+        _starts(what, dq_out, dk_out, q, k, dq, dk, q_weight, k_weight)
+        _on_gpu(q)
+        return (_strides(dq_out, dk_out, q, k, dq, dk), _L().a2v_qk_norm_rope_workspace(*p[-1]), *p)
+    st, need, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections),
+                                                   (q, k, q_weight, k_weight, inv_freq, pos, dq_out, dk_out, dq_weight, dk_weight, *((dq, dk) if given else ())), plan)
     if dq_weight.data_ptr() == dk_weight.data_ptr():
-        raise ValueError("qk_norm_rope_bwd: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
+        raise ValueError(f"{what}: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
     if given:
-        _results("qk_norm_rope_bwd", (("dq", dq, q), ("dk", dk, k)))
-        _apart("qk_norm_rope_bwd", (dq, dk), (dq_out, dk_out, q, k), (dq_out, dk_out))
+        _apart(what, (dq, dk), (dq_out, dk_out, q, k), (dq_out, dk_out))
     if q.numel() == 0:
         return dq, dk
-    need = _L().a2v_qk_norm_rope_workspace(N, S, H, HK, HD)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _on_device(_L().a2v_qk_norm_rope_bwd,
-               (dt(q), ptr(dq_out), ptr(dk_out), ptr(q), ptr(k), ptr(dq), ptr(dk), _strides(dq_out, dk_out, q, k, dq, dk), ptr(q_weight), ptr(k_weight),
-                ptr(dq_weight), ptr(dk_weight), ptr(args[0]), ptr(args[1]), *args[2:], 1 if interleaved else 0, float(eps), N, S, H, HK, HD, ptr(ws), need), q, "a2v_qk_norm_rope_bwd")
+    _run(_L().a2v_qk_norm_rope_bwd, "a2v_qk_norm_rope_bwd", q.device, code, *_starts(what, dq_out, dk_out, q, k, dq, dk), st, *_starts(what, q_weight, k_weight),
+         dq_weight.data_ptr(), dk_weight.data_ptr(), inv_freq.data_ptr(), None if pos is None else pos.data_ptr(), ps, axes, sec,
+         1 if interleaved else 0, eps, *sizes, ws.data_ptr(), need)
     return dq, dk
 
 
-def _linear_attention_args(what, q, k, v, slopes, state, cu_seqlens):
+def _linear_attention_checks(what, q, k, v, slopes, state, cu_seqlens):
+    """-> B, S, H, HK, HD"""
     if _HALF and q.dtype == torch.float16:
         raise TypeError(f"{what}: not built for float16 (a state does not fit its range); use bfloat16 or float32")
     _heads(f"{what}: q", q, 4)
@@ -748,21 +808,30 @@ def linear_attention_fwd(q, k, v, slopes, *, scale=None, state=None, cu_seqlens=
     cu_seqlens (B+1) int32 on the device: q, k, v are (1,T,heads,HD) and sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1], which may
     be none; rows outside every sequence are zeros in a result of this call's own and left as they were in the caller's `out`.
     The products take 16-bit operands as pairs: sums, scores and states keep fp32 accuracy, out is rounded once."""
-    B, S, H, HK, HD = _linear_attention_args("linear_attention_fwd", q, k, v, slopes, state, cu_seqlens)
-    own = out is None
-    if own:
-        out = _E(*q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _results("linear_attention_fwd", (("out", out, q),))
-        _apart("linear_attention_fwd", (out,), (q, k, v))
-    last = _E(B, H, HD, HD, dtype=torch.float32, device=q.device) if want_state else None
+    what = "linear_attention_fwd"
+    given = out is not None
+    if not given:
+        out = _like(q)
+
+    def plan():
+        sizes = _linear_attention_checks(what, q, k, v, slopes, state, cu_seqlens)
+        _results(what, (("out", out, q),))
+        if given:
+            _apart(what, (out,), (q, k, v))
+        _starts(what, q, k, v, out)
+        _on_gpu(q)
+        return dt(q), _strides(q, k, v, out), sizes, _L().a2v_linear_attention_workspace(dt(q), 0, cu_seqlens is not None, *sizes)
+    code, st, sizes, need = _layout(what, None, (q, k, v, slopes, state, cu_seqlens, out if given else None), plan)
+    if given:
+        _apart(what, (out,), (q, k, v))
+    B, _, H, _, HD = sizes
+    last = torch.empty((B, H, HD, HD), dtype=torch.float32, device=q.device) if want_state else None
     if B == 0:
         return out, last
-    need = _L().a2v_linear_attention_workspace(dt(q), 0, cu_seqlens is not None, B, S, H, HK, HD)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _on_device(_L().a2v_linear_attention_fwd,
-               (dt(q), ptr(q), ptr(k), ptr(v), ptr(out), _strides(q, k, v, out), ptr(slopes), ptr(state), ptr(last), ptr(cu_seqlens), B, S, H, HK, HD,
-                float(HD ** -0.5 if scale is None else scale), 1 if own else 0, ptr(ws), need), q, "a2v_linear_attention_fwd")
+    _run(_L().a2v_linear_attention_fwd, "a2v_linear_attention_fwd", q.device, code, *_starts(what, q, k, v, out), st, slopes.data_ptr(),
+         None if state is None else state.data_ptr(), None if last is None else last.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+         *sizes, HD ** -0.5 if scale is None else scale, 0 if given else 1, None if ws is None else ws.data_ptr(), need)
     return out, last
 
 
@@ -770,28 +839,35 @@ def linear_attention_bwd(q, k, v, slopes, d_out, *, scale=None, state=None, d_st
     """-> dq, dk, dv and the gradient of `state` (None without one).  d_state: gradient of the state behind the last row, or None.
     dq, dk, dv: all three (views of a packed gradient, for instance) or none; rows outside every sequence as in linear_attention_fwd.
     Gradients of a shared k / v head are summed over its heads in fp32; nothing here depends on the order of arrival."""
-    B, S, H, HK, HD = _linear_attention_args("linear_attention_bwd", q, k, v, slopes, state, cu_seqlens)
-    _results("linear_attention_bwd", (("d_out", d_out, q),), out=False)
-    if d_state is not None:
-        _f32("linear_attention_bwd: d_state", d_state, (B, H, HD, HD), q)
-    given = [t is not None for t in (dq, dk, dv)]
-    if any(given) and not all(given):
-        raise ValueError("linear_attention_bwd: dq, dk and dv come together or not at all")
-    own = not any(given)
-    if own:
-        dq, dk, dv = (_E(*t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    else:
-        _results("linear_attention_bwd", (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)))
-        _apart("linear_attention_bwd", (dq, dk, dv), (q, k, v, d_out))
-    first = _E(B, H, HD, HD, dtype=torch.float32, device=q.device) if state is not None else None
-    if B == 0:
+    what = "linear_attention_bwd"
+    given = dq is not None or dk is not None or dv is not None
+    if given and (dq is None or dk is None or dv is None):
+        raise ValueError(f"{what}: dq, dk and dv come together or not at all")
+    if not given:
+        dq, dk, dv = _like(q), _like(k), _like(v)
+
+    def plan():
+        sizes = _linear_attention_checks(what, q, k, v, slopes, state, cu_seqlens)
+        _results(what, (("d_out", d_out, q),), out=False)
+        _results(what, (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)))
+        if d_state is not None:
+            _f32(f"{what}: d_state", d_state, (sizes[0], sizes[2], sizes[4], sizes[4]), q)
+        if given:
+            _apart(what, (dq, dk, dv), (q, k, v, d_out))
+        _starts(what, q, k, v, d_out, dq, dk, dv)
+        _on_gpu(q)
+        return dt(q), _strides(q, k, v, d_out, dq, dk, dv), sizes, _L().a2v_linear_attention_workspace(dt(q), 1, cu_seqlens is not None, *sizes)
+    code, st, sizes, need = _layout(what, None, (q, k, v, slopes, d_out, state, d_state, cu_seqlens, *((dq, dk, dv) if given else ())), plan)
+    if given:
+        _apart(what, (dq, dk, dv), (q, k, v, d_out))
+    first = None if state is None else torch.empty_like(state)
+    if sizes[0] == 0:
         return dq, dk, dv, first
-    need = _L().a2v_linear_attention_workspace(dt(q), 1, cu_seqlens is not None, B, S, H, HK, HD)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _on_device(_L().a2v_linear_attention_bwd,
-               (dt(q), ptr(q), ptr(k), ptr(v), ptr(d_out), ptr(dq), ptr(dk), ptr(dv), _strides(q, k, v, d_out, dq, dk, dv), ptr(slopes), ptr(state),
-                ptr(d_state), ptr(first), ptr(cu_seqlens), B, S, H, HK, HD, float(HD ** -0.5 if scale is None else scale), 1 if own else 0,
-                ptr(ws), need), q, "a2v_linear_attention_bwd")
+    _run(_L().a2v_linear_attention_bwd, "a2v_linear_attention_bwd", q.device, code, *_starts(what, q, k, v, d_out, dq, dk, dv), st, slopes.data_ptr(),
+         None if state is None else state.data_ptr(), None if d_state is None else d_state.data_ptr(), None if first is None else first.data_ptr(),
+         None if cu_seqlens is None else cu_seqlens.data_ptr(), *sizes, sizes[4] ** -0.5 if scale is None else scale, 0 if given else 1,
+         None if ws is None else ws.data_ptr(), need)
     return dq, dk, dv, first
 
 
@@ -800,31 +876,40 @@ def linear_attention_step(q, k, v, slopes, state, *, slots=None, scale=None, out
     slots (N) int32 on the device: the pool entry of each row (default row n).  Rows that name the same entry are successive rows of
     one stream, in order; an entry outside the pool touches no state and gives zeros (padding rows of a captured graph)."""
     what = "linear_attention_step"
-    _heads(f"{what}: q", q, 3)
-    _heads(f"{what}: k", k, 3, q)
-    _heads(f"{what}: v", v, 3, q)
-    N, H, HD = q.shape
-    HK = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != N or k.shape[2] != HD or H < 1 or HK < 1 or H % HK:
-        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    _f32(f"{what}: slopes", slopes, (H,), q)
-    _f32(f"{what}: state", state, (state.shape[0], H, HD, HD), q)
-    if slots is None:
-        if state.shape[0] < N:
-            raise ValueError(f"{what}: {N} rows and {state.shape[0]} states")
-    elif slots.dtype != torch.int32 or slots.device != q.device or tuple(slots.shape) != (N,) or not slots.is_contiguous():
-        raise ValueError(f"{what}: slots int32 ({N},) on {q.device} expected, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
-    if out is None:
-        out = _E(N, H, HD, dtype=q.dtype, device=q.device)
-    else:
+    given = out is not None
+    if not given:
+        out = _like(q)
+
+    def plan():
+        _heads(f"{what}: q", q, 3)
+        _heads(f"{what}: k", k, 3, q)
+        _heads(f"{what}: v", v, 3, q)
+        N, H, HD = q.shape
+        if k.shape != v.shape or k.shape[0] != N or k.shape[2] != HD or H < 1 or k.shape[1] < 1 or H % k.shape[1]:
+            raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+        _f32(f"{what}: slopes", slopes, (H,), q)
+        _f32(f"{what}: state", state, (state.shape[0], H, HD, HD), q)
+        if slots is None:
+            if state.shape[0] < N:
+                raise ValueError(f"{what}: {N} rows and {state.shape[0]} states")
+        elif slots.dtype != torch.int32 or slots.device != q.device or tuple(slots.shape) != (N,) or not slots.is_contiguous():
+            raise ValueError(f"{what}: slots int32 ({N},) on {q.device} expected, got {slots.dtype} {tuple(slots.shape)} on {slots.device}")
         _results(what, (("out", out, q),))
+        if given:
+            _apart(what, (out,), (q, k, v))
+        _starts(what, q, k, v, out)
+        _on_gpu(q)
+        st = (C.c_longlong * 8)(*[s if n > 1 else 0 for t in (q, k, v, out) for s, n in zip(t.stride()[:2], t.shape)])
+        return dt(q), st, (state.shape[0], N, H, k.shape[1], HD, HD ** -0.5)
+    code, st, sizes = _layout(what, None, (q, k, v, slopes, state, slots, out if given else None), plan)
+    if given:
         _apart(what, (out,), (q, k, v))
-    if N == 0:
+    if sizes[1] == 0:
         return out
-    st = (C.c_longlong * 8)(*[s if n > 1 else 0 for t in (q, k, v, out) for s, n in zip(t.stride()[:2], t.shape)])
-    _on_device(_L().a2v_linear_attention_step,
-               (dt(q), ptr(q), ptr(k), ptr(v), ptr(out), st, ptr(slopes), ptr(state), ptr(slots), state.shape[0], N, H, HK, HD,
-                float(HD ** -0.5 if scale is None else scale)), q, "a2v_linear_attention_step")
+    if scale is not None:
+        sizes = (*sizes[:5], scale)
+    _run(_L().a2v_linear_attention_step, "a2v_linear_attention_step", q.device, code, *_starts(what, q, k, v, out), st, slopes.data_ptr(), state.data_ptr(),
+         None if slots is None else slots.data_ptr(), *sizes)
     return out
 
 
