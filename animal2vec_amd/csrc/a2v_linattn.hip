@@ -16,13 +16,22 @@
 // state nor the scores ever pass through LDS; the price is that every wave forms the chunk's scores itself.
 // Products are issued swapped (P^T = K Q^T, O^T = V^T P^T + Y^T Q^T): see a2v_attn.hip for the layout argument.
 //
-// 16-bit runs: scores, the scaled values and the state go into the matrix cores as hi + lo pairs (two products each, 2^-17 relative),
-// because one 16-bit rounding of each would add up to more than the one rounding of the result that the type asks for.
+// All products run on the bf16 matrix cores, fp32 values as sums of bf16 parts of 8 bits each (x = hi + mid + lo exactly; the products of
+// parts are exact in the fp32 accumulators):
+//   bf16 operands: q, k, v are one part; scores and the state two (2^-16 relative), the scaled values two, or three where the state is
+//     a result.  One rounding of each to 16 bits would add up to more than the one rounding of the result that the type asks for.
+//   fp32 operands: three parts of everything, six products of parts (the three below 2^-24 are dropped): 96 matrix cycles for 32 channels
+//     of a 16 x 16 tile where v_mfma_f32_16x16x4_f32 takes 256.
 #include "a2v_common.h"
 
 typedef __attribute__((address_space(3))) s16x4 la_lds_s16x4;
+// bfloat16 in both libraries: scores and states have its range, not half's
+typedef __attribute__((ext_vector_type(2))) __bf16 lb2;
+typedef __attribute__((ext_vector_type(4))) __bf16 lb4;
+typedef __attribute__((ext_vector_type(8))) __bf16 lb8;
 
 typedef __attribute__((ext_vector_type(4))) unsigned lin_raw;     // 16 bytes in flight
+typedef __attribute__((ext_vector_type(2))) unsigned lin_half;
 
 struct LinRole {
   const void* q; const void* k; const void* v; void* o;
@@ -50,94 +59,93 @@ struct LinArgs {
   int roles, roles_state, split;                                 // roles of the main and of the state kernel; the axis is cut into segments
 };
 
+#define LIN_C 32              /* rows of a chunk: two tiles of 16 */
 template <typename T> struct LinT;
-template <> struct LinT<bf16> {
-  static constexpr int C = 32, V = 8;                            // rows of a chunk, elements of a 16-byte load
-  static constexpr bool SPLIT = true;
-  typedef bf16x8 frag;
-  static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, const f32x4& c) { return A2V_MFMA_16x16x32(a, b, c, 0, 0, 0); }
-};
-template <> struct LinT<float> {
-  static constexpr int C = 32, V = 4;                            // fp32 MFMA runs at 1/16 of the rate: half the chunk, half the scores
-  static constexpr bool SPLIT = false;
-  struct frag { float e[8]; __device__ __forceinline__ float& operator[](int i) { return e[i]; } __device__ __forceinline__ float operator[](int i) const { return e[i]; } };
-  static __device__ __forceinline__ f32x4 mma(const frag& a, const frag& b, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], c, 0, 0, 0);
-    return c;
-  }
-};
+template <> struct LinT<__bf16> { static constexpr int IN = 1, MID = 2, V = 8; };      // parts of the operands, of scores and states; elements of 16 bytes
+template <> struct LinT<float> { static constexpr int IN = 3, MID = 3, V = 4; };
 
-// A tile is C rows of HD elements at a pitch of HD elements + 16 bytes: both the row reads (16 rows, 8 or 16 bytes each) and the
-// transposed reads (4 rows x 32 bytes, or 4 rows x 16 words) then touch every bank once.
-template <typename T, int HD> __device__ __forceinline__ constexpr int lin_pitch() { return HD + 16 / (int)sizeof(T); }
-
-// 8 elements of row `r` at columns {32 kd + 4 g ..+3} and {32 kd + 16 + 4 g ..+3}: the order the state's accumulator tiles have
-template <typename T, int HD> __device__ __forceinline__ typename LinT<T>::frag lin_row(const T* tile, int r, int kd, int g) {
-  const T* p = tile + r * lin_pitch<T, HD>() + 32 * kd + 4 * g;
-  typename LinT<T>::frag f;
-  if constexpr (LinT<T>::SPLIT) {
-    const bf16x4 a = *(const bf16x4*)p, b = *(const bf16x4*)(p + 16);
+// x[0 .. 2 N - 1] = the sum of PARTS bf16 parts: the nearest, the nearest to what is left, and so on; two elements at a time (v_cvt_pk,
+// then a shift and a mask to get the pair back: 6 instructions a pair and part)
+template <int PARTS, int N> __device__ __forceinline__ void lin_split(const float* x, unsigned (&w)[PARTS][N]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[4 + i] = b[i]; }
-  } else {
-    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 16);
+  for (int i = 0; i < N; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[i] = a[i]; f[4 + i] = b[i]; }
-  }
-  return f;
-}
-// the transpose: column `c0 + lane % 16`, rows {32 ks + 4 g ..+3} and {32 ks + 16 + 4 g ..+3}
-template <typename T, int HD> __device__ __forceinline__ typename LinT<T>::frag lin_col(const T* tile, int ks, int c0, int lane) {
-  typename LinT<T>::frag f;
-  const int g = lane >> 4;
-  constexpr int P = lin_pitch<T, HD>();
-  if constexpr (LinT<T>::SPLIT) {
-    const T* p = tile + (32 * ks + 4 * g + ((lane & 15) >> 2)) * P + c0 + 4 * (lane & 3);
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)p);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)(p + 16 * P));
-    union { struct { s16x4 a, b; } s; bf16x8 v; } u;
-    u.s.a = a; u.s.b = b;
-    f = u.v;
-  } else {
-    const T* p = tile + (32 * ks + 4 * g) * P + c0 + (lane & 15);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[i] = p[i * P]; f[4 + i] = p[(16 + i) * P]; }
-  }
-  return f;
-}
-// x = hi + lo (+ lo2): the nearest 16-bit value, the nearest to what is left, and so on; two elements at a time (v_cvt_pk, then a shift
-// and a mask to get the pair back: 6 instructions a pair and part)
-template <typename T, int PARTS> __device__ __forceinline__ void lin_split(const float* x, typename LinT<T>::frag* f) {
-  if constexpr (LinT<T>::SPLIT) {
-    union { unsigned w[4]; bf16x8 v; } u[PARTS];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a = x[2 * i], b = x[2 * i + 1];
-#pragma unroll
-      for (int k = 0; k < PARTS; ++k) {
-        const bf16x2 h = __builtin_convertvector((f32x2){a, b}, bf16x2);
-        u[k].w[i] = __builtin_bit_cast(unsigned, h);
-        if (k + 1 < PARTS) { a -= a2v_lo16_f32(u[k].w[i]); b -= a2v_hi16_f32(u[k].w[i]); }
-      }
+    for (int k = 0; k < PARTS; ++k) {
+      w[k][i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, lb2));
+      if (k + 1 < PARTS) { a -= __builtin_bit_cast(float, w[k][i] << 16); b -= __builtin_bit_cast(float, w[k][i] & 0xffff0000u); }
     }
-#pragma unroll
-    for (int k = 0; k < PARTS; ++k) f[k] = u[k].v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[0][i] = x[i];
   }
 }
+template <int PARTS> __device__ __forceinline__ void lin_split8(const float* x, lb8 (&f)[PARTS]) {
+  union { unsigned w[PARTS][4]; lb8 v[PARTS]; } u;
+  lin_split<PARTS, 4>(x, u.w);
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) f[k] = u.v[k];
+}
+// c += a b over 32 of the inner index, a and b in parts; products below the last part of the longer one are left out
+template <int NA, int NB> __device__ __forceinline__ f32x4 lin_mma(const lb8 (&a)[NA], const lb8 (&b)[NB], f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j < (NA > NB ? NA : NB)) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c, 0, 0, 0);
+  return c;
+}
 
-// S += k^T x over 32 rows of the tile, x (the wave's 16 columns, weighted) in PARTS 16-bit parts
-template <typename T, int HD, int PARTS> __device__ __forceinline__ void lin_update(f32x4* S, const float* x, const T* sK, int ks, int lane) {
-  typename LinT<T>::frag p[PARTS];
-  lin_split<T, PARTS>(x, p);
+// A tile in LDS is its parts, each LIN_C rows of HD bf16 at a pitch of HD elements + 16 bytes.
+template <typename T, int HD> struct LinTile {
+  static constexpr int IN = LinT<T>::IN, PITCH = 2 * HD + 16, PART = LIN_C * PITCH, BYTES = IN * PART;
+  static __device__ __forceinline__ void put(char* tile, int r, int c, lin_raw x) {            // 16 bytes, piece c of row r
+    if constexpr (IN == 1) *(lin_raw*)(tile + r * PITCH + 16 * c) = x;
+    else {
+      const f32x4 f = __builtin_bit_cast(f32x4, x);
+      const float e[4] = {f[0], f[1], f[2], f[3]};
+      unsigned w[IN][2];
+      lin_split<IN, 2>(e, w);
+#pragma unroll
+      for (int k = 0; k < IN; ++k) *(lin_half*)(tile + k * PART + r * PITCH + 8 * c) = (lin_half){w[k][0], w[k][1]};
+    }
+  }
+  // 8 elements of row r at columns {32 kd + 4 g ..+3} and {32 kd + 16 + 4 g ..+3}: the order the state's accumulator tiles have
+  static __device__ __forceinline__ void row(const char* tile, int r, int kd, int g, lb8 (&f)[IN]) {
+#pragma unroll
+    for (int k = 0; k < IN; ++k) {
+      const char* const p = tile + k * PART + r * PITCH + 64 * kd + 8 * g;
+      const lb4 a = *(const lb4*)p, b = *(const lb4*)(p + 32);
+      f[k] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // the transpose: column 16 ct + lane % 16, rows {4 g ..+3} and {16 + 4 g ..+3}
+  static __device__ __forceinline__ void col(const char* tile, int ct, int lane, lb8 (&f)[IN]) {
+#pragma unroll
+    for (int k = 0; k < IN; ++k) {
+      const char* const p = tile + k * PART + (4 * (lane >> 4) + ((lane & 15) >> 2)) * PITCH + 32 * ct + 8 * (lane & 3);
+      union { struct { s16x4 a, b; } s; lb8 v; } u;
+      u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)p);
+      u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)(p + 16 * PITCH));
+      f[k] = u.v;
+    }
+  }
+};
+template <int IN> __device__ __forceinline__ float lin_value(const lb8 (&f)[IN], int i) {       // the element that the parts stand for
+  float x = (float)f[0][i];
+#pragma unroll
+  for (int k = 1; k < IN; ++k) x += (float)f[k][i];
+  return x;
+}
+__device__ __forceinline__ void lin_store4(float* p, const f32x4& v) { *(f32x4*)p = v; }
+__device__ __forceinline__ void lin_store4(__bf16* p, const f32x4& v) { *(lb4*)p = __builtin_convertvector(v, lb4); }
+
+// S += k^T x over the tile's rows, x (the wave's 16 columns, weighted) in PARTS parts
+template <typename T, int HD, int PARTS> __device__ __forceinline__ void lin_update(f32x4 (&S)[HD / 16], const float (&x)[8], const char* sK, int lane) {
+  lb8 p[PARTS];
+  lin_split8<PARTS>(x, p);
 #pragma unroll
   for (int t = 0; t < HD / 16; ++t) {
-    const typename LinT<T>::frag kf = lin_col<T, HD>(sK, ks, 16 * t, lane);
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i) S[t] = LinT<T>::mma(kf, p[i], S[t]);
+    lb8 kf[LinT<T>::IN];
+    LinTile<T, HD>::col(sK, t, lane, kf);
+    S[t] = lin_mma(kf, p, S[t]);
   }
 }
 
@@ -177,17 +185,17 @@ __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amd
 
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 template <typename T, int HD, bool STATE>
-__global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) void lin_kernel(LinArgs a) {
+__global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
-  typedef typename L::frag frag;
-  constexpr int C = L::C, NT = C / 16, NS = C / 32, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, P = lin_pitch<T, HD>();
+  typedef LinTile<T, HD> Tile;
+  constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = HD * (int)sizeof(T) + 16;       // OP: pitch of the result's tile, bytes
   constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
-  __shared__ __attribute__((aligned(16))) T sm[STATE ? 2 : 4][C * P];
-  T* const sK = sm[0];
-  T* const sV = sm[1];
-  T* const sQ = sm[STATE ? 0 : 2];
-  T* const sO = sm[STATE ? 0 : 3];
+  __shared__ __attribute__((aligned(16))) char sm[(STATE ? 2 : 3) * Tile::BYTES + (STATE ? 0 : C * OP)];
+  char* const sK = sm;
+  char* const sV = sm + Tile::BYTES;
+  char* const sQ = sm + (STATE ? 0 : 2) * Tile::BYTES;
+  char* const sO = sm + (STATE ? 0 : 3) * Tile::BYTES;
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
   const int nr = STATE ? a.roles_state : a.roles, nin = nr * a.rep, HK = a.H / a.rep;
@@ -290,10 +298,10 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
   auto place = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int c = tid + u * THREADS, at = (c / CPR) * P + (c % CPR) * L::V;
-      if constexpr (!STATE) *(lin_raw*)(sQ + at) = pq[u];
-      *(lin_raw*)(sK + at) = pk[u];
-      *(lin_raw*)(sV + at) = pv[u];
+      const int at = tid + u * THREADS, i = at / CPR, e = at % CPR;
+      if constexpr (!STATE) Tile::put(sQ, i, e, pq[u]);
+      Tile::put(sK, i, e, pk[u]);
+      Tile::put(sV, i, e, pv[u]);
     }
   };
 
@@ -307,7 +315,7 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
     w1[i] = scale * lin_pow(l2, 16 + d);
     wv[i] = r.s_state * lin_pow(l2, 16 - 4 * g - i);
   }
-  const float l16 = lin_uniform(lin_pow(l2, 16)), l32 = lin_uniform(lin_pow(l2, 32)), l48 = lin_uniform(lin_pow(l2, 48)), lrow = r.s_inter * lin_pow(l2, fr);
+  const float l16 = lin_uniform(lin_pow(l2, 16)), lrow = r.s_inter * lin_pow(l2, fr);
 
   offsets_in(C);
   if constexpr (!STATE) offsets(ao, r.os, C);
@@ -318,52 +326,45 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
     __syncthreads();
     if (t0 + C < upto) fetch(t0 + C);
 
-    frag vf[NS];
-#pragma unroll
-    for (int ks = 0; ks < NS; ++ks) vf[ks] = lin_col<T, HD>(sV, ks, n0, lane);
+    lb8 vf[L::IN];
+    Tile::col(sV, n0 / 16, lane, vf);
     if constexpr (!STATE) {
-      frag y[NK][L::SPLIT ? 2 : 1];
+      lb8 y[NK][L::MID];
 #pragma unroll
       for (int kd = 0; kd < NK; ++kd) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
-        lin_split<T, L::SPLIT ? 2 : 1>(x, y[kd]);
+        lin_split8<L::MID>(x, y[kd]);
       }
-      float f = lrow;
 #pragma unroll
-      for (int ti = 0; ti < NT; ++ti) {                          // one tile of 16 query rows at a time (registers: see the launch bounds)
-        frag qf[NK];
+      for (int ti = 0; ti < 2; ++ti) {                           // a tile of 16 query rows
+        lb8 qf[NK][L::IN];
         f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kd = 0; kd < NK; ++kd) {
-          qf[kd] = lin_row<T, HD>(sQ, 16 * ti + fr, kd, g);
-          acc = L::mma(y[kd][0], qf[kd], acc);
-          if constexpr (L::SPLIT) acc = L::mma(y[kd][1], qf[kd], acc);
+          Tile::row(sQ, 16 * ti + fr, kd, g, qf[kd]);
+          acc = lin_mma(y[kd], qf[kd], acc);
         }
-        acc *= f;
-        f *= l16;
+        float x[8];
 #pragma unroll
-        for (int ks = 0; 2 * ks <= ti; ++ks) {
-          float x[8];
+        for (int e = 0; e < 2; ++e) {                            // against the keys of tile e <= ti
+          f32x4 p = (f32x4){0.f, 0.f, 0.f, 0.f};
+          if (e <= ti)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = ti - 2 * ks - e;                       // tiles between the queries and the keys
-            f32x4 p = (f32x4){0.f, 0.f, 0.f, 0.f};
-            if (d >= 0)
+            for (int kd = 0; kd < NK; ++kd) {
+              lb8 kf[L::IN];
+              Tile::row(sK, 16 * e + fr, kd, g, kf);
+              p = lin_mma(kf, qf[kd], p);
+            }
 #pragma unroll
-              for (int kd = 0; kd < NK; ++kd) p = L::mma(lin_row<T, HD>(sK, 32 * ks + 16 * e + fr, kd, g), qf[kd], p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              // on the diagonal a select, not a product: a non-finite key does not reach the rows in front of it
-              x[4 * e + i] = d < 0 ? 0.f : d == 0 ? (fr < 4 * g + i ? 0.f : p[i] * w0[i]) : (d == 1 ? p[i] : p[i] * (d == 2 ? l16 : l32)) * w1[i];
-          }
-          frag p[L::SPLIT ? 2 : 1];
-          lin_split<T, L::SPLIT ? 2 : 1>(x, p);
-          acc = L::mma(vf[ks], p[0], acc);
-          if constexpr (L::SPLIT) acc = L::mma(vf[ks], p[1], acc);
+          for (int i = 0; i < 4; ++i)                            // on the diagonal a select, not a product: a non-finite key stays behind
+            x[4 * e + i] = e > ti ? 0.f : e == ti ? (fr < 4 * g + i ? 0.f : p[i] * w0[i]) : p[i] * w1[i];
         }
-        if (!r.o32) Vec4<T>::store(sO + (16 * ti + fr) * P + n0 + 4 * g, acc);
+        lb8 p[L::MID];
+        lin_split8<L::MID>(x, p);
+        acc = lin_mma(vf, p, acc * (ti ? lrow * l16 : lrow));
+        if (!r.o32) lin_store4((T*)(sO + (16 * ti + fr) * OP) + n0 + 4 * g, acc);
         else {
           const int t = t0 + 16 * ti + fr;
           if (t < upto) *(f32x4*)(oF + (a.cu ? 0 : b * r.on) + (long long)(row0 + dir * t) * r.os + (long long)h * r.oh + n0 + 4 * g) = acc;
@@ -376,28 +377,25 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
       const float le = lin_pow(l2, e);
 #pragma unroll
       for (int t = 0; t < ND; ++t) S[t] *= le;
+      float x[8];
+      if (e == C) {                                              // l^(C - j), j = 16 tile + 4 g + i
 #pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {
-        float x[8];
-        if (e == C) {                                            // l^(C - j), j = 16 tile + 4 g + i: a factor of the lane and one of the tile
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int up = NT - 1 - 2 * ks - (i >> 2);           // tiles behind this one
-            x[i] = ((float)vf[ks][i] * (up == 0 ? 1.f : up == 1 ? l16 : up == 2 ? l32 : l48)) * wv[i & 3];
-          }
-        } else {
-          int j0 = 4 * g;
-          asm volatile("" : "+v"(j0));                           // (keeps 16 lane constants of this rare branch out of the loop's registers)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int j = j0 + 32 * ks + 16 * (i >> 2) + (i & 3);
-            x[i] = j < c ? (float)vf[ks][i] * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
-          }
+        for (int i = 0; i < 4; ++i) {
+          x[i] = lin_value(vf, i) * l16 * wv[i];
+          x[4 + i] = lin_value(vf, 4 + i) * wv[i];
         }
-        // a state that leaves the call (or might: out does not depend on that) keeps its 32 bits, three parts of 8; else two do
-        if (L::SPLIT && r.exact) lin_update<T, HD, L::SPLIT ? 3 : 1>(S, x, sK, ks, lane);
-        else lin_update<T, HD, L::SPLIT ? 2 : 1>(S, x, sK, ks, lane);
+      } else {
+        int j0 = 4 * g;
+        asm volatile("" : "+v"(j0));                             // (keeps the lane constants of this rare branch out of the loop's registers)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = j0 + 16 * (i >> 2) + (i & 3);
+          x[i] = j < c ? lin_value(vf, i) * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
+        }
       }
+      // a state that leaves the call (or might: out does not depend on that) keeps its 32 bits, three parts of 8; else two do
+      if (L::MID < 3 && r.exact) lin_update<T, HD, 3>(S, x, sK, lane);
+      else lin_update<T, HD, L::MID>(S, x, sK, lane);
     }
     __syncthreads();
     if constexpr (!STATE) {
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(HD * 4, HD == 128 ? 2 : LinT<T>::SPLIT ? 4 : 3) voi
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           const int at = tid + u * THREADS;
-          if (at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (at / CPR) * P + (at % CPR) * L::V), (lin_raw*)(bo + ao[u]));
+          if (at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (at / CPR) * OP + (at % CPR) * 16), (lin_raw*)(bo + ao[u]));
         }
       }
     }
@@ -476,8 +474,8 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* dk32, const 
     const float* q = dv32 + (row * H + hk * rep) * HD + d;
     for (int u = 0; u < rep; ++u) { a += *(const f32x4*)(p + u * HD); c += *(const f32x4*)(q + u * HD); }
   }
-  Vec4<T>::store(dk + n * kn + t * ks + hk * kh + d, a);
-  Vec4<T>::store(dv + n * vn + t * vs + hk * vh + d, c);
+  lin_store4(dk + n * kn + t * ks + hk * kh + d, a);
+  lin_store4(dv + n * vn + t * vs + hk * vh + d, c);
 }
 
 // One token of each of N streams, the state updated in place: state once in, once out, everything else is negligible (HBM, or latency
@@ -559,7 +557,7 @@ static int lin_seg(int B, long long rows, int S, int H, int HD, bool packed, int
 }
 struct LinPlan { int C, seg, slots; bool split; size_t states; };
 static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPlan& p) {
-  p.C = dtype == A2V_F32 ? LinT<float>::C : LinT<bf16>::C;
+  p.C = LIN_C;
   const long long rows = packed ? S : (long long)B * S;
   if (rows >= (1LL << 30)) return false;
   p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
@@ -628,7 +626,7 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
   a.r[1] = a.r[2] = r;
   a.roles = a.roles_state = 1; a.split = p.split; a.rep = H / HK;
   if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
-  else lin_launch<bf16>(a, p, HD, stream);
+  else lin_launch<__bf16>(a, p, HD, stream);
   A2V_CHECK_LAUNCH();
   return A2V_OK;
 }
@@ -669,14 +667,14 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
     for (int i = 0; i < 2; ++i) { g[i]->o = to[i]; g[i]->on = pn; g[i]->os = ps; g[i]->oh = HD; g[i]->o32 = 1; }
   }
   if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
-  else lin_launch<bf16>(a, p, HD, stream);
+  else lin_launch<__bf16>(a, p, HD, stream);
   if (rep > 1 && rows) {
     const dim3 grid((unsigned)cdiv((long)(rows * HK * HD / 4), 256));
     if (dtype == A2V_F32)
       hipLaunchKernelGGL(lin_join_kernel<float>, grid, dim3(256), 0, stream, dk32, dv32, (float*)dk, (float*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
                          cu_seqlens, B, S, S, H, rep, HD, a.fill);
     else
-      hipLaunchKernelGGL(lin_join_kernel<bf16>, grid, dim3(256), 0, stream, dk32, dv32, (bf16*)dk, (bf16*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
+      hipLaunchKernelGGL(lin_join_kernel<__bf16>, grid, dim3(256), 0, stream, dk32, dv32, (__bf16*)dk, (__bf16*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
                          cu_seqlens, B, S, S, H, rep, HD, a.fill);
   }
   A2V_CHECK_LAUNCH();
