@@ -23,6 +23,7 @@
 //   fp32 operands: three parts of everything, six products of parts (the three below 2^-24 are dropped): 96 matrix cycles for 32 channels
 //     of a 16 x 16 tile where v_mfma_f32_16x16x4_f32 takes 256.
 #include "a2v_common.h"
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) s16x4 la_lds_s16x4;
 // bfloat16 in both libraries: scores and states have its range, not half's
@@ -33,10 +34,10 @@ typedef __attribute__((ext_vector_type(8))) __bf16 lb8;
 typedef __attribute__((ext_vector_type(4))) unsigned lin_raw;     // 16 bytes in flight
 typedef __attribute__((ext_vector_type(2))) unsigned lin_half;
 
+struct LinOperand { const char* p; long long n, s, h; };        // address; bytes between sequences, rows, heads
 struct LinRole {
-  const void* q; const void* k; const void* v; void* o;
-  long long qn, qs, qh, kn, ks, kh, vn, vs, vh, on, os, oh;     // strides in elements: sequence, row, head
-  int qr, kr, vr;                                                // heads that share one head of the operand
+  LinOperand q, k, v, o;
+  int shared;                                                    // operands of HK heads: bit 0 q, bit 1 k, bit 2 v
   int reverse;                                                   // rows are visited from the last to the first
   int first_t;                                                   // `first` is read transposed
   int ws_t;                                                      // so are the segment states: they are another role's
@@ -52,12 +53,13 @@ struct LinArgs {
   const float* slopes;
   const int* cu;                                                 // (B + 1) row offsets, or null: B sequences of S rows
   int B, S, H, T;                                                // T: rows in all (cu), S: rows of a sequence
-  int seg;                                                       // rows of a segment, a multiple of the chunk
+  int seg, np;                                                   // rows of a segment, a multiple of the chunk; segments of a sequence (no cu)
   int slots;
   int fill;                                                      // rows outside every sequence become 0 (cu)
-  int rep;                                                       // heads that share one head of k and v
+  int rep, HK;                                                   // heads that share one head of k and v; those heads
   int roles, roles_state, split;                                 // roles of the main and of the state kernel; the axis is cut into segments
 };
+#define LIN_GRID_Y 32768
 
 #define LIN_C 32              /* rows of a chunk: two tiles of 16 */
 template <typename T> struct LinT;
@@ -137,18 +139,6 @@ template <int IN> __device__ __forceinline__ float lin_value(const lb8 (&f)[IN],
 __device__ __forceinline__ void lin_store4(float* p, const f32x4& v) { *(f32x4*)p = v; }
 __device__ __forceinline__ void lin_store4(__bf16* p, const f32x4& v) { *(lb4*)p = __builtin_convertvector(v, lb4); }
 
-// S += k^T x over the tile's rows, x (the wave's 16 columns, weighted) in PARTS parts
-template <typename T, int HD, int PARTS> __device__ __forceinline__ void lin_update(f32x4 (&S)[HD / 16], const float (&x)[8], const char* sK, int lane) {
-  lb8 p[PARTS];
-  lin_split8<PARTS>(x, p);
-#pragma unroll
-  for (int t = 0; t < HD / 16; ++t) {
-    lb8 kf[LinT<T>::IN];
-    LinTile<T, HD>::col(sK, t, lane, kf);
-    S[t] = lin_mma(kf, p, S[t]);
-  }
-}
-
 // slot -> (sequence, segment).  Sequences start wherever cu says, so sequence b gets the slots floor(start / seg) + b ...: that many are
 // always enough (ceil(len / seg) <= floor((start + len) / seg) - floor(start / seg) + 1), none is shared, and their number is known to
 // the host without reading cu.  Offsets are clamped to [0, T]: a wrong cu gives wrong rows, never an access outside the tensors.
@@ -156,18 +146,17 @@ struct LinSeq { int b, p, np, begin, len; };                     // begin: first
 __device__ __forceinline__ int lin_cu(const LinArgs& a, int b) { const int c = a.cu[b]; return c < 0 ? 0 : (c > a.T ? a.T : c); }
 __device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) {
   if (!a.cu) {
-    s.np = a.S > a.seg ? (a.S + a.seg - 1) / a.seg : 1;
-    s.b = slot / s.np;
-    s.p = slot - s.b * s.np;
+    s.np = a.np;
+    s.b = a.np == 1 ? slot : slot / a.np;
+    s.p = slot - s.b * a.np;
     s.begin = 0;
     s.len = a.S;
-    return s.b < a.B;
+    return true;
   }
-  int lo = 0, hi = a.B;                                          // the last b in [0, B) whose first slot is <= slot
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (lin_cu(a, mid) / a.seg + mid <= slot) lo = mid; else hi = mid;
-  }
+  int lo = -1;                                                   // the last b in [0, B) whose first slot is <= slot: the slots ascend, so count
+  for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) < a.B; i += 64)       // (64 sequences a look: a binary search is six loads in a row)
+    lo += __popcll(__ballot(i < a.B && lin_cu(a, i) / a.seg + i <= slot));
+  lo = lo < 0 ? 0 : lo;
   s.b = lo;
   s.begin = lin_cu(a, lo);
   const int end = lin_cu(a, lo + 1);
@@ -198,18 +187,17 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
   char* const sO = sm + (STATE ? 0 : 3) * Tile::BYTES;
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
-  const int nr = STATE ? a.roles_state : a.roles, nin = nr * a.rep, HK = a.H / a.rep;
-  const int grp = blockIdx.x / (8 * nin), rem = blockIdx.x - grp * 8 * nin, in = rem >> 3, unit = grp * 8 + (rem & 7);
-  const int slot0 = unit / HK, h = (unit - slot0 * HK) * a.rep + in / nr;
+  const int nr = STATE ? a.roles_state : a.roles, in = blockIdx.x >> 3, unit = (blockIdx.z * LIN_GRID_Y + blockIdx.y) * 8 + (blockIdx.x & 7);
+  const int of = nr == 1 ? in : nr == 2 ? in >> 1 : in * 21846 >> 16;         // in / nr (in < 3 * 4096)
+  const int slot0 = unit / a.HK, hk = unit - slot0 * a.HK, h = hk * a.rep + of;
   if (slot0 >= a.slots) return;
-  const LinRole& r = a.r[in % nr];
+  const LinRole r = a.r[in - of * nr];                           // by value: its fields in a few wide loads, not one by one where they are used
   // the main kernel of a split axis starts with the last segments: their k and v are what the state kernel has read last
   const int slot = !STATE && a.split ? a.slots - 1 - slot0 : slot0;
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, n0 = (tid >> 6) * 16;
   LinSeq s;
   const bool mine = lin_find(a, slot, s);
-  T* const oT = (T*)r.o;
-  float* const oF = (float*)r.o;
+  char* const out = (char*)r.o.p + h * r.o.h;
   if constexpr (!STATE) {
     if (a.fill) {                                                // rows in front of the first and behind the last sequence
       int z0 = 0, z1 = 0;
@@ -217,8 +205,8 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
       if (behind >= 0) { z0 = cB + behind * a.seg; z1 = z0 + a.seg < a.T ? z0 + a.seg : a.T; }
       else if (slot <= c0 / a.seg) { z0 = slot * a.seg; z1 = z0 + a.seg < c0 ? z0 + a.seg : c0; }
       for (long long i = tid; i < (long long)(z1 - z0) * HD; i += THREADS) {
-        const long long at = (z0 + i / HD) * r.os + (long long)h * r.oh + i % HD;
-        if (r.o32) oF[at] = 0.f; else oT[at] = (T)0.f;
+        char* const at = out + (z0 + i / HD) * r.o.s;
+        if (r.o32) ((float*)at)[i % HD] = 0.f; else ((T*)at)[i % HD] = (T)0.f;
       }
     }
   }
@@ -230,6 +218,61 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
   const bool ends = s.p == s.np - 1;                             // this workgroup meets the sequence's last position
   const float l2 = lin_log2(a.slopes, h);
   const int off = r.reverse ? 0 : 1;                             // `first` is S_0 forward (Y = l S_0) and Y itself backwards
+
+  // A chunk's c rows lie in a row of memory, backwards in a reverse role: each operand is a uniform address that moves by a chunk, and an
+  // offset per 16-byte piece that only the last chunk changes.  Its missing rows are copies of the last one (what they hold meets a zero
+  // weight).  (Forming the addresses from the row number again in every chunk, with their 64-bit products and the reads of the strides,
+  // took 10 % of a chunk's time.)
+  const bool rev = r.reverse;
+  const int row0 = rev ? s.begin + s.len - 1 : s.begin, dir = rev ? -1 : 1;        // row of position t: row0 + dir * t
+  const int low = rev ? row0 - from - (C - 1) : row0 + from;
+  const long long qs = r.q.s, ks = r.k.s, vs = r.v.s, os = r.o.s, n = a.cu ? 0 : b;
+  const char* bq = r.q.p + n * r.q.n + (r.shared & 1 ? hk : h) * r.q.h + low * qs;
+  const char* bk = r.k.p + n * r.k.n + (r.shared & 2 ? hk : h) * r.k.h + low * ks;
+  const char* bv = r.v.p + n * r.v.n + (r.shared & 4 ? hk : h) * r.v.h + low * vs;
+  char* bo = out + n * r.o.n + low * os;
+  const long long dq = qs * (dir * C), dk = ks * (dir * C), dv = vs * (dir * C), dO = os * (dir * C);
+  const bool o32 = r.o32;
+  lin_raw pq[NU], pk[NU], pv[NU];                                // the next chunk's tiles, in flight during this one's math
+  unsigned aq[NU], ak[NU], av[NU], ao[NU];
+  auto offsets = [&](unsigned (&off)[NU], long long stride, int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int at = tid + u * THREADS, i = at / CPR < c ? at / CPR : c - 1;
+      off[u] = (unsigned)(rev ? c - 1 - i : i) * (unsigned)stride + (at % CPR) * 16;
+    }
+  };
+  auto offsets_in = [&](int c) __attribute__((always_inline)) {
+    if constexpr (!STATE) offsets(aq, qs, c);
+    offsets(ak, ks, c);
+    offsets(av, vs, c);
+  };
+  auto fetch = [&](int c) __attribute__((always_inline)) {
+    if (c < C) {
+      offsets_in(c);
+      if (rev) { bq += (C - c) * qs; bk += (C - c) * ks; bv += (C - c) * vs; }
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if constexpr (!STATE) pq[u] = *(const lin_raw*)(bq + aq[u]);
+      pk[u] = *(const lin_raw*)(bk + ak[u]);
+      pv[u] = *(const lin_raw*)(bv + av[u]);
+    }
+    bq += dq; bk += dk; bv += dv;
+  };
+  auto place = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int at = tid + u * THREADS, i = at / CPR, e = at % CPR;
+      if constexpr (!STATE) Tile::put(sQ, i, e, pq[u]);
+      Tile::put(sK, i, e, pk[u]);
+      Tile::put(sV, i, e, pv[u]);
+    }
+  };
+
+  offsets_in(C);
+  if constexpr (!STATE) offsets(ao, os, C);
+  if (from < upto) fetch(upto - from < C ? upto - from : C);
 
   f32x4 S[ND];                                                   // S[t][i]: row 16 t + 4 g + i of the state, column n0 + fr
 #pragma unroll
@@ -258,53 +301,6 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
     }
   }
 
-  const T* const q = (const T*)r.q + (a.cu ? 0 : b * r.qn) + (long long)(h / r.qr) * r.qh;
-  const T* const k = (const T*)r.k + (a.cu ? 0 : b * r.kn) + (long long)(h / r.kr) * r.kh;
-  const T* const v = (const T*)r.v + (a.cu ? 0 : b * r.vn) + (long long)(h / r.vr) * r.vh;
-  T* const oB = oT + (a.cu ? 0 : b * r.on) + (long long)h * r.oh;
-  const int row0 = r.reverse ? s.begin + s.len - 1 : s.begin, dir = r.reverse ? -1 : 1;      // row of position t: row0 + dir * t
-
-  // A tile's rows t0 .. t0 + c - 1 lie at row `low` and above, in reverse order backwards: a uniform address and an offset per piece that
-  // only the last chunk changes.  Its missing rows are copies of the last one (whatever they hold meets a zero weight).
-  lin_raw pq[NU], pk[NU], pv[NU];                                 // the next chunk's tiles, in flight during this one's math
-  unsigned aq[NU], ak[NU], av[NU], ao[NU];
-  auto offsets = [&](unsigned (&off)[NU], long long stride, int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int at = tid + u * THREADS, i = at / CPR < c ? at / CPR : c - 1;
-      off[u] = (unsigned)(r.reverse ? c - 1 - i : i) * (unsigned)(stride * sizeof(T)) + (at % CPR) * 16;
-    }
-  };
-  auto offsets_in = [&](int c) __attribute__((always_inline)) {
-    if constexpr (!STATE) offsets(aq, r.qs, c);
-    offsets(ak, r.ks, c);
-    offsets(av, r.vs, c);
-  };
-  auto low = [&](int t0, int c) { return (long long)(r.reverse ? row0 - t0 - (c - 1) : row0 + t0); };
-  auto fetch = [&](int t0) __attribute__((always_inline)) {
-    const int c = upto - t0 < C ? upto - t0 : C;
-    const long long n = low(t0, c);
-    const char* const bq = (const char*)(q + n * r.qs);
-    const char* const bk = (const char*)(k + n * r.ks);
-    const char* const bv = (const char*)(v + n * r.vs);
-    if (c < C) offsets_in(c);
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      if constexpr (!STATE) pq[u] = *(const lin_raw*)(bq + aq[u]);
-      pk[u] = *(const lin_raw*)(bk + ak[u]);
-      pv[u] = *(const lin_raw*)(bv + av[u]);
-    }
-  };
-  auto place = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int at = tid + u * THREADS, i = at / CPR, e = at % CPR;
-      if constexpr (!STATE) Tile::put(sQ, i, e, pq[u]);
-      Tile::put(sK, i, e, pk[u]);
-      Tile::put(sV, i, e, pv[u]);
-    }
-  };
-
   // l^(i - j) scale for a query column fr and key rows 4 g + i: inside a tile, and one tile apart
   const float scale = r.s_inter * r.s_state;
   float w0[4], w1[4], wv[4];
@@ -315,19 +311,19 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
     w1[i] = scale * lin_pow(l2, 16 + d);
     wv[i] = r.s_state * lin_pow(l2, 16 - 4 * g - i);
   }
-  const float l16 = lin_uniform(lin_pow(l2, 16)), lrow = r.s_inter * lin_pow(l2, fr);
+  const bool exact = r.exact;
+  const float l16 = lin_uniform(lin_pow(l2, 16)), lC = lin_uniform(lin_pow(l2, C)), lrow = r.s_inter * lin_pow(l2, fr);
 
-  offsets_in(C);
-  if constexpr (!STATE) offsets(ao, r.os, C);
-  if (from < upto) fetch(from);
-  for (int t0 = from; t0 < upto; t0 += C) {
-    const int c = upto - t0 < C ? upto - t0 : C;
+  // one chunk of c rows; END: the segment's last one, which may be short and may end the sequence
+  auto chunk = [&](auto end, int t0, int c) __attribute__((always_inline)) {
+    constexpr bool END = decltype(end)::value;
     place();
     __syncthreads();
-    if (t0 + C < upto) fetch(t0 + C);
-
+    if constexpr (!END) fetch(upto - t0 - C < C ? upto - t0 - C : C);
     lb8 vf[L::IN];
     Tile::col(sV, n0 / 16, lane, vf);
+    f32x4 acc[2];                                                // results of the two query tiles
+    acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if constexpr (!STATE) {
       lb8 y[NK][L::MID];
 #pragma unroll
@@ -337,81 +333,104 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
         for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
         lin_split8<L::MID>(x, y[kd]);
       }
+      f32x4 pt[3];                                               // scores of the tiles (queries, keys) = (0, 0), (1, 0), (1, 1)
 #pragma unroll
-      for (int ti = 0; ti < 2; ++ti) {                           // a tile of 16 query rows
-        lb8 qf[NK][L::IN];
-        f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 3; ++i) pt[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kd = 0; kd < NK; ++kd) {
-          Tile::row(sQ, 16 * ti + fr, kd, g, qf[kd]);
-          acc = lin_mma(y[kd], qf[kd], acc);
-        }
+      for (int kd = 0; kd < NK; ++kd) {
+        lb8 q0[L::IN], q1[L::IN], k0[L::IN], k1[L::IN];
+        Tile::row(sQ, fr, kd, g, q0);
+        Tile::row(sQ, 16 + fr, kd, g, q1);
+        Tile::row(sK, fr, kd, g, k0);
+        Tile::row(sK, 16 + fr, kd, g, k1);
+        pt[0] = lin_mma(k0, q0, pt[0]);
+        pt[1] = lin_mma(k0, q1, pt[1]);
+        pt[2] = lin_mma(k1, q1, pt[2]);
+        acc[0] = lin_mma(y[kd], q0, acc[0]);
+        acc[1] = lin_mma(y[kd], q1, acc[1]);
+      }
+#pragma unroll
+      for (int ti = 0; ti < 2; ++ti) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                            // against the keys of tile e <= ti
-          f32x4 p = (f32x4){0.f, 0.f, 0.f, 0.f};
-          if (e <= ti)
-#pragma unroll
-            for (int kd = 0; kd < NK; ++kd) {
-              lb8 kf[L::IN];
-              Tile::row(sK, 16 * e + fr, kd, g, kf);
-              p = lin_mma(kf, qf[kd], p);
-            }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)                            // on the diagonal a select, not a product: a non-finite key stays behind
-            x[4 * e + i] = e > ti ? 0.f : e == ti ? (fr < 4 * g + i ? 0.f : p[i] * w0[i]) : p[i] * w1[i];
+        for (int i = 0; i < 4; ++i) {                            // on the diagonal a select, not a product: a non-finite key stays behind
+          x[i] = ti ? pt[1][i] * w1[i] : fr < 4 * g + i ? 0.f : pt[0][i] * w0[i];
+          x[4 + i] = !ti || fr < 4 * g + i ? 0.f : pt[2][i] * w0[i];
         }
         lb8 p[L::MID];
         lin_split8<L::MID>(x, p);
-        acc = lin_mma(vf, p, acc * (ti ? lrow * l16 : lrow));
-        if (!r.o32) lin_store4((T*)(sO + (16 * ti + fr) * OP) + n0 + 4 * g, acc);
-        else {
-          const int t = t0 + 16 * ti + fr;
-          if (t < upto) *(f32x4*)(oF + (a.cu ? 0 : b * r.on) + (long long)(row0 + dir * t) * r.os + (long long)h * r.oh + n0 + 4 * g) = acc;
-        }
+        acc[ti] = lin_mma(vf, p, acc[ti] * (ti ? lrow * l16 : lrow));
       }
     }
-    const bool last = ends && t0 + C >= upto;
-    if (!last || r.last) {
-      const int e = last ? c - off : c;                          // the state behind the last row itself, or as the next row sees it
-      const float le = lin_pow(l2, e);
+    if (!END || !ends || r.last) {
+      const int e = END && ends ? c - off : C;                   // the state behind the last row itself, or as the next row sees it
+      const float le = END ? lin_pow(l2, e) : lC;
 #pragma unroll
       for (int t = 0; t < ND; ++t) S[t] *= le;
       float x[8];
-      if (e == C) {                                              // l^(C - j), j = 16 tile + 4 g + i
+      if (!END || e == C) {                                      // l^(C - j), j = 16 tile + 4 g + i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[i] = lin_value(vf, i) * l16 * wv[i];
           x[4 + i] = lin_value(vf, 4 + i) * wv[i];
         }
       } else {
-        int j0 = 4 * g;
-        asm volatile("" : "+v"(j0));                             // (keeps the lane constants of this rare branch out of the loop's registers)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int j = j0 + 16 * (i >> 2) + (i & 3);
+          const int j = 4 * g + 16 * (i >> 2) + (i & 3);
           x[i] = j < c ? lin_value(vf, i) * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
         }
       }
-      // a state that leaves the call (or might: out does not depend on that) keeps its 32 bits, three parts of 8; else two do
-      if (L::MID < 3 && r.exact) lin_update<T, HD, 3>(S, x, sK, lane);
-      else lin_update<T, HD, L::MID>(S, x, sK, lane);
+      // two parts of the weighted values; a state that leaves the call (or might: out does not depend on that) keeps its 32 bits with a third
+      lb8 p[3];
+      lin_split8<3>(x, p);
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        lb8 kf[L::IN], m[L::MID];
+#pragma unroll
+        for (int i = 0; i < L::MID; ++i) m[i] = p[i];
+        Tile::col(sK, t, lane, kf);
+        S[t] = lin_mma(kf, m, S[t]);
+      }
+      if (L::MID < 3 && exact)
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          lb8 kf[L::IN];
+          Tile::col(sK, t, lane, kf);
+          S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[0], p[2], S[t], 0, 0, 0);
+        }
+    }
+    if constexpr (!STATE) {
+#pragma unroll
+      for (int ti = 0; ti < 2; ++ti) {
+        if (!o32) lin_store4((T*)(sO + (16 * ti + fr) * OP) + n0 + 4 * g, acc[ti]);
+        else {
+          const int t = t0 + 16 * ti + fr;
+          if (t < upto) *(f32x4*)(out + n * r.o.n + (long long)(row0 + dir * t) * os + (n0 + 4 * g) * 4) = acc[ti];
+        }
+      }
     }
     __syncthreads();
     if constexpr (!STATE) {
       // whole rows, 16 bytes a lane: 8-byte pieces straight from the accumulators cost 10 % of the launch.  Past the L2, which the
       // operands need: 2 to 5 % on every long case.
-      if (!r.o32) {
-        char* const bo = (char*)(oB + low(t0, c) * r.os);
-        if (c < C) offsets(ao, r.os, c);
+      if (!o32) {
+        if (END && c < C) {
+          offsets(ao, os, c);
+          if (rev) bo += (C - c) * os;
+        }
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           const int at = tid + u * THREADS;
-          if (at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (at / CPR) * OP + (at % CPR) * 16), (lin_raw*)(bo + ao[u]));
+          if (!END || at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (at / CPR) * OP + (at % CPR) * 16), (lin_raw*)(bo + ao[u]));
         }
+        bo += dO;
       }
     }
-  }
+  };
+  int t0 = from;
+  for (; t0 + C < upto; t0 += C) chunk(std::false_type{}, t0, C);
+  if (t0 < upto) chunk(std::true_type{}, t0, upto - t0);
   if constexpr (STATE) {
     f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
 #pragma unroll
@@ -425,10 +444,11 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
   }
 }
 
-// ws[slot] := the state in front of segment p from the segments before it: carried through the sequence's slots in order, one thread per
-// four elements (any order of them: the waves' register image).  The part of `first` is added by the kernel that starts from it.
+// ws[slot] := the state in front of segment p from the segments before it: carried through the sequence's slots in order, one thread to an
+// element (any order of them: the waves' register image), eight loads in flight.  The part of `first` is added by the kernel that starts
+// from it.
 __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
-  const int b = blockIdx.y;
+  const int per = a.H * HH / 256, b = blockIdx.x / per;
   LinSeq s;
   if (a.cu) {
     s.begin = lin_cu(a, b);
@@ -438,21 +458,20 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
   s.np = s.len > a.seg ? (s.len + a.seg - 1) / a.seg : 1;
   if (s.np < 2) return;
   const int slot0 = a.cu ? s.begin / a.seg + b : b * s.np;
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;       // element of (H, HD, HD); HD * HD % 1024 == 0
-  const int h = (int)(i / HH);
+  const int i = (blockIdx.x - b * per) * 256 + threadIdx.x, h = i / HH;        // element of (H, HD, HD); HD * HD % 256 == 0
   const float f = lin_pow(lin_log2(a.slopes, h), a.seg);
-  f32x4* w = (f32x4*)(a.r[blockIdx.z].ws + (long long)slot0 * a.H * HH + i);
-  const long long step = (long long)a.H * HH / 4;
-  f32x4 carry = {0.f, 0.f, 0.f, 0.f};
+  const long long step = (long long)a.H * HH;
+  float* const w = a.r[blockIdx.y].ws + slot0 * step + i;
+  float carry = 0.f;
   int p = 0;
-  for (; p + 4 < s.np; p += 4) {                                 // four loads in flight (the last segment has no state of its own)
-    f32x4 x[4];
+  for (; p + 8 < s.np; p += 8) {                                 // (the last segment has no state of its own)
+    float x[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = w[(p + u) * step];
+    for (int u = 0; u < 8; ++u) x[u] = w[(p + u) * step];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) { w[(p + u) * step] = carry; carry = carry * f + x[u]; }
+    for (int u = 0; u < 8; ++u) { w[(p + u) * step] = carry; carry = carry * f + x[u]; }
   }
-  for (; p < s.np - 1; ++p) { const f32x4 x = w[p * step]; w[p * step] = carry; carry = carry * f + x; }
+  for (; p < s.np - 1; ++p) { const float x = w[p * step]; w[p * step] = carry; carry = carry * f + x; }
   w[p * step] = carry;
 }
 
@@ -562,29 +581,32 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
   if (rows >= (1LL << 30)) return false;
   p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
   const long long slots = packed ? (long long)S / p.seg + B + 1 : (long long)B * (S > p.seg ? (S + p.seg - 1) / p.seg : 1);
-  if ((slots + 8) * H * 3 >= (1LL << 31)) return false;
+  if ((slots + 8) * H * 3 >= (1LL << 31) || (long long)B * H * HD * HD / 256 >= (1LL << 31)) return false;
   p.slots = (int)slots;
   p.split = S > p.seg;
   p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
   return true;
 }
 static bool lin_shape_ok(int B, int S, int H, int HK, int HD) {
-  return B >= 0 && S >= 0 && H > 0 && HK > 0 && H % HK == 0 && H <= 65535 && B <= 65535 * 16 && (HD == 32 || HD == 64 || HD == 128);
+  return B >= 0 && S >= 0 && H > 0 && HK > 0 && H % HK == 0 && H / HK <= 1024 && (HD == 32 || HD == 64 || HD == 128);
 }
 static bool lin_tensor_ok(const void* p, const long long* st, int es) {
   return p && !((uintptr_t)p & 15) && !((st[0] * es) & 15) && !((st[1] * es) & 15) && !((st[2] * es) & 15) && st[1] >= 0 &&
          st[1] * es < (1 << 26);                                 // (offsets inside a chunk are 32 bits)
 }
 
+static dim3 lin_grid(const LinArgs& a, int roles) {
+  const unsigned groups = (unsigned)(((long long)a.slots * a.HK + 7) / 8);
+  return dim3(8 * roles * a.rep, groups < LIN_GRID_Y ? groups : LIN_GRID_Y, (groups + LIN_GRID_Y - 1) / LIN_GRID_Y);
+}
 template <typename T, int HD>
 static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
-  const long long n = ((long long)p.slots * (a.H / a.rep) + 7) / 8 * 8 * a.rep;
   const dim3 block(HD * 4);
   if (p.split) {
-    hipLaunchKernelGGL((lin_kernel<T, HD, true>), dim3((unsigned)(n * a.roles_state)), block, 0, stream, a);
-    hipLaunchKernelGGL(lin_scan_kernel, dim3(a.H * HD * HD / 1024, a.B, a.roles_state), dim3(256), 0, stream, a, HD * HD);
+    hipLaunchKernelGGL((lin_kernel<T, HD, true>), lin_grid(a, a.roles_state), block, 0, stream, a);
+    hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)((long long)a.H * HD * HD / 256 * a.B), a.roles_state), dim3(256), 0, stream, a, HD * HD);
   }
-  hipLaunchKernelGGL((lin_kernel<T, HD, false>), dim3((unsigned)(n * a.roles)), block, 0, stream, a);
+  hipLaunchKernelGGL((lin_kernel<T, HD, false>), lin_grid(a, a.roles), block, 0, stream, a);
 }
 template <typename T>
 static void lin_launch(const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {
@@ -598,6 +620,13 @@ static int lin_dtype(int dtype) {
   if (dtype == A2V_BF16) return A2V_ERR_UNSUPPORTED;             // states and scores have bf16's range, not half's (65504)
 #endif
   return A2V_OK;
+}
+
+static LinOperand lin_op(const void* p, const long long* st, int es) { return LinOperand{(const char*)p, st[0] * es, st[1] * es, st[2] * es}; }
+static void lin_args(LinArgs& a, const LinPlan& p, const float* slopes, const int* cu, int B, int S, int H, int HK, int zero_outside) {
+  a.slopes = slopes; a.cu = cu; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu && zero_outside;
+  a.np = S > p.seg ? (S + p.seg - 1) / p.seg : 1;
+  a.HK = HK; a.rep = H / HK; a.split = p.split;
 }
 
 extern "C" size_t a2v_linear_attention_workspace(int dtype, int backward, int packed, int B, int S, int H, int HK, int HD) {
@@ -619,12 +648,12 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
     return A2V_ERR_ARG;
   if (p.states > ws_bytes || (p.states && (!ws || ((uintptr_t)ws & 15)))) return A2V_ERR_ARG;
   LinArgs a;
-  a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
-  LinRole& r = a.r[0];
-  r = LinRole{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10],
-              strides[11], 1, H / HK, H / HK, 0, 0, 0, 1, 0, scale, 1.f, state, state_out, (float*)ws};
-  a.r[1] = a.r[2] = r;
-  a.roles = a.roles_state = 1; a.split = p.split; a.rep = H / HK;
+  lin_args(a, p, slopes, cu_seqlens, B, S, H, HK, zero_outside);
+  const int kv = H != HK ? 6 : 0;
+  a.r[0] = LinRole{lin_op(q, strides, es), lin_op(k, strides + 3, es), lin_op(v, strides + 6, es), lin_op(out, strides + 9, es),
+                   kv, 0, 0, 0, 1, 0, scale, 1.f, state, state_out, (float*)ws};
+  a.r[1] = a.r[2] = a.r[0];
+  a.roles = a.roles_state = 1;
   if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
   else lin_launch<__bf16>(a, p, HD, stream);
   A2V_CHECK_LAUNCH();
@@ -650,31 +679,30 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
   const size_t rows = cu_seqlens ? (size_t)S : (size_t)B * S;
   float* const dk32 = (float*)(w + 2 * p.states);
   float* const dv32 = dk32 + rows * H * HD;
-  const long long* const s = strides;
-  const long long pn = (long long)S * H * HD, ps = (long long)H * HD;
   LinArgs a;
-  a.slopes = slopes; a.cu = cu_seqlens; a.B = B; a.S = S; a.H = H; a.T = S; a.seg = p.seg; a.slots = p.slots; a.fill = cu_seqlens && zero_outside;
-  a.r[0] = LinRole{d_out, v, k, dq, s[9], s[10], s[11], s[6], s[7], s[8], s[3], s[4], s[5], s[12], s[13], s[14],
-                   1, rep, rep, 0, 1, 0, 0, 0, scale, 1.f, state, nullptr, (float*)w};
-  a.roles = 3; a.roles_state = 2; a.split = p.split; a.rep = rep;               // dk's segment states are the transposes of dv's
-  a.r[1] = LinRole{k, q, d_out, dv, s[3], s[4], s[5], s[0], s[1], s[2], s[9], s[10], s[11], s[18], s[19], s[20],
-                   rep, 1, 1, 1, 0, 0, d_state != nullptr, 0, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
-  a.r[2] = LinRole{v, d_out, q, dk, s[6], s[7], s[8], s[9], s[10], s[11], s[0], s[1], s[2], s[15], s[16], s[17],
-                   rep, 1, 1, 1, 1, 1, 0, 0, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
-  if (rep > 1) {
-    LinRole* const g[2] = {&a.r[1], &a.r[2]};
-    float* const to[2] = {dv32, dk32};
-    for (int i = 0; i < 2; ++i) { g[i]->o = to[i]; g[i]->on = pn; g[i]->os = ps; g[i]->oh = HD; g[i]->o32 = 1; }
+  lin_args(a, p, slopes, cu_seqlens, B, S, H, HK, zero_outside);
+  LinOperand o[7];
+  for (int i = 0; i < 7; ++i) o[i] = lin_op(t[i], strides + 3 * i, es);
+  LinOperand &Q = o[0], &K = o[1], &V = o[2], &D = o[3], gk = o[5], gv = o[6];
+  if (rep > 1) {                                                 // fp32 rows of every head, summed behind the kernel
+    const long long one[3] = {(long long)S * H * HD, (long long)H * HD, HD};
+    gk = lin_op(dk32, one, 4);
+    gv = lin_op(dv32, one, 4);
   }
+  const int o32 = rep > 1, kv = rep > 1;
+  a.r[0] = LinRole{D, V, K, o[4], 6 * kv, 0, 1, 0, 0, 0, scale, 1.f, state, nullptr, (float*)w};
+  a.r[1] = LinRole{K, Q, D, gv, kv, 1, 0, 0, d_state != nullptr, o32, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
+  a.r[2] = LinRole{V, D, Q, gk, kv, 1, 1, 1, 0, o32, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
+  a.roles = 3; a.roles_state = 2;                                // dk's segment states are the transposes of dv's
   if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
   else lin_launch<__bf16>(a, p, HD, stream);
   if (rep > 1 && rows) {
     const dim3 grid((unsigned)cdiv((long)(rows * HK * HD / 4), 256));
     if (dtype == A2V_F32)
-      hipLaunchKernelGGL(lin_join_kernel<float>, grid, dim3(256), 0, stream, dk32, dv32, (float*)dk, (float*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
+      hipLaunchKernelGGL(lin_join_kernel<float>, grid, dim3(256), 0, stream, dk32, dv32, (float*)dk, (float*)dv, strides[15], strides[16], strides[17], strides[18], strides[19], strides[20],
                          cu_seqlens, B, S, S, H, rep, HD, a.fill);
     else
-      hipLaunchKernelGGL(lin_join_kernel<__bf16>, grid, dim3(256), 0, stream, dk32, dv32, (__bf16*)dk, (__bf16*)dv, s[15], s[16], s[17], s[18], s[19], s[20],
+      hipLaunchKernelGGL(lin_join_kernel<__bf16>, grid, dim3(256), 0, stream, dk32, dv32, (__bf16*)dk, (__bf16*)dv, strides[15], strides[16], strides[17], strides[18], strides[19], strides[20],
                          cu_seqlens, B, S, S, H, rep, HD, a.fill);
   }
   A2V_CHECK_LAUNCH();
