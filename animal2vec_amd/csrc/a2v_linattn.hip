@@ -174,17 +174,19 @@ __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amd
 
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 template <typename T, int HD, bool STATE>
-__global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(LinArgs a) {
+__global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
   typedef LinTile<T, HD> Tile;
   constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = HD * (int)sizeof(T) + 16;       // OP: pitch of the result's tile, bytes
   constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
-  __shared__ __attribute__((aligned(16))) char sm[(STATE ? 2 : 3) * Tile::BYTES + (STATE ? 0 : C * OP)];
+  constexpr int WAVES = HD / 16, PP = 72, PPART = C * PP;        // scores: 32 rows of 32 bf16 at a pitch of 18 words (16 rows, 16 lanes: all banks)
+  __shared__ __attribute__((aligned(16))) char sm[(STATE ? 2 : 3) * Tile::BYTES + (STATE ? 0 : C * OP + L::MID * PPART)];
   char* const sK = sm;
   char* const sV = sm + Tile::BYTES;
   char* const sQ = sm + (STATE ? 0 : 2) * Tile::BYTES;
   char* const sO = sm + (STATE ? 0 : 3) * Tile::BYTES;
+  char* const sP = sO + (STATE ? 0 : C * OP);
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
   const int nr = STATE ? a.roles_state : a.roles, in = blockIdx.x >> 3, unit = (blockIdx.z * LIN_GRID_Y + blockIdx.y) * 8 + (blockIdx.x & 7);
@@ -195,6 +197,8 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
   // the main kernel of a split axis starts with the last segments: their k and v are what the state kernel has read last
   const int slot = !STATE && a.split ? a.slots - 1 - slot0 : slot0;
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, n0 = (tid >> 6) * 16;
+  // which score tiles this wave forms: the first of three waves changes from workgroup to workgroup (a wave stays on its SIMD)
+  const int mine_p = (__builtin_amdgcn_readfirstlane(tid >> 6) + blockIdx.y) % WAVES;
   LinSeq s;
   const bool mine = lin_find(a, slot, s);
   char* const out = (char*)r.o.p + h * r.o.h;
@@ -320,48 +324,48 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
     place();
     __syncthreads();
     if constexpr (!END) fetch(upto - t0 - C < C ? upto - t0 - C : C);
-    lb8 vf[L::IN];
-    Tile::col(sV, n0 / 16, lane, vf);
     f32x4 acc[2];                                                // results of the two query tiles
     acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if constexpr (!STATE) {
-      lb8 y[NK][L::MID];
+      // the scores of the tiles (queries, keys) = (0, 0), (1, 0), (1, 1), one wave to a tile, for all waves: in LDS, in parts
+#pragma unroll
+      for (int n = 0; n < 3; ++n)
+        if (n % (WAVES < 3 ? WAVES : 3) == mine_p) {
+          const int ti = n > 0, e = n > 1;
+          f32x4 p = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kd = 0; kd < NK; ++kd) {
+            lb8 qf[L::IN], kf[L::IN];
+            Tile::row(sQ, 16 * ti + fr, kd, g, qf);
+            Tile::row(sK, 16 * e + fr, kd, g, kf);
+            p = lin_mma(kf, qf, p);
+          }
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)                            // on the diagonal a select, not a product: a non-finite key stays behind
+            x[i] = n == 1 ? p[i] * w1[i] : fr < 4 * g + i ? 0.f : p[i] * w0[i];
+          unsigned w[L::MID][2];
+          lin_split<L::MID, 2>(x, w);
+#pragma unroll
+          for (int k = 0; k < L::MID; ++k) *(lin_half*)(sP + k * PPART + (16 * ti + fr) * PP + 32 * e + 8 * g) = (lin_half){w[k][0], w[k][1]};
+        }
 #pragma unroll
       for (int kd = 0; kd < NK; ++kd) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
-        lin_split8<L::MID>(x, y[kd]);
-      }
-      f32x4 pt[3];                                               // scores of the tiles (queries, keys) = (0, 0), (1, 0), (1, 1)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) pt[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kd = 0; kd < NK; ++kd) {
-        lb8 q0[L::IN], q1[L::IN], k0[L::IN], k1[L::IN];
+        lb8 y[L::MID], q0[L::IN], q1[L::IN];
+        lin_split8<L::MID>(x, y);
         Tile::row(sQ, fr, kd, g, q0);
         Tile::row(sQ, 16 + fr, kd, g, q1);
-        Tile::row(sK, fr, kd, g, k0);
-        Tile::row(sK, 16 + fr, kd, g, k1);
-        pt[0] = lin_mma(k0, q0, pt[0]);
-        pt[1] = lin_mma(k0, q1, pt[1]);
-        pt[2] = lin_mma(k1, q1, pt[2]);
-        acc[0] = lin_mma(y[kd], q0, acc[0]);
-        acc[1] = lin_mma(y[kd], q1, acc[1]);
+        acc[0] = lin_mma(y, q0, acc[0]);
+        acc[1] = lin_mma(y, q1, acc[1]);
       }
-#pragma unroll
-      for (int ti = 0; ti < 2; ++ti) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {                            // on the diagonal a select, not a product: a non-finite key stays behind
-          x[i] = ti ? pt[1][i] * w1[i] : fr < 4 * g + i ? 0.f : pt[0][i] * w0[i];
-          x[4 + i] = !ti || fr < 4 * g + i ? 0.f : pt[2][i] * w0[i];
-        }
-        lb8 p[L::MID];
-        lin_split8<L::MID>(x, p);
-        acc[ti] = lin_mma(vf, p, acc[ti] * (ti ? lrow * l16 : lrow));
-      }
+      acc[0] *= lrow;
+      acc[1] *= lrow * l16;
     }
+    lb8 vf[L::IN];
+    Tile::col(sV, n0 / 16, lane, vf);
     if (!END || !ends || r.last) {
       const int e = END && ends ? c - off : C;                   // the state behind the last row itself, or as the next row sees it
       const float le = END ? lin_pow(l2, e) : lC;
@@ -399,6 +403,20 @@ __global__ __launch_bounds__(HD * 4, HD == 128 || LinT<T>::IN > 1 ? 2 : 4) void 
           Tile::col(sK, t, lane, kf);
           S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[0], p[2], S[t], 0, 0, 0);
         }
+    }
+    if constexpr (!STATE) {
+      __syncthreads();
+#pragma unroll
+      for (int ti = 0; ti < 2; ++ti) {
+        lb8 p[L::MID];
+#pragma unroll
+        for (int k = 0; k < L::MID; ++k) {
+          const char* const at = sP + k * PPART + (16 * ti + fr) * PP + 8 * g;
+          const lb4 lo = *(const lb4*)at, hi = ti ? *(const lb4*)(at + 32) : (lb4){};
+          p[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        acc[ti] = lin_mma(vf, p, acc[ti]);
+      }
     }
     if constexpr (!STATE) {
 #pragma unroll
