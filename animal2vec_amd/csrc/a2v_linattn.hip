@@ -582,13 +582,15 @@ __global__ __launch_bounds__(256) void lin_step_kernel(LinStep a) {
 #define LIN_WGS 1024          /* workgroups that fill the card: four on each of 256 CUs */
 
 // Rows of a segment.  Enough (sequence, head) pairs: one segment each, k and v read once.  Fewer: the axis is cut until LIN_WGS
-// workgroups run, which costs a second pass over k and v; not below 4 HD rows, where the states (HD * HD * 4 bytes, written and read)
-// would weigh as much as those rows.
+// workgroups run, which costs a second pass over k and v; not below 4 HD rows, where writing and reading the states (HD * HD * 4 bytes)
+// costs as much as it gives (4 clips of 2000 rows, 16 heads: 34.4 us at 256 rows, 36.4 at 128), except that fewer than a workgroup for
+// each compute unit are worse still: then 2 HD (one such clip: 26.8 us at 256 rows, 23.6 at 128, 24.9 at 64).
 static int lin_seg(int B, long long rows, int S, int H, int HD, bool packed, int C) {
   const long long all = packed ? rows : S;
   if (!packed && (long long)B * H >= LIN_WGS / 2) return all > 0 ? cdiv(all, C) * C : C;
   long long seg = (rows * H + LIN_WGS - 1) / LIN_WGS;
-  if (seg < 4 * HD) seg = 4 * HD;
+  const int least = rows * H < 256LL * 4 * HD ? 2 * HD : 4 * HD;
+  if (seg < least) seg = least;
   if (seg > all) seg = all;
   return seg < C ? C : cdiv(seg, C) * C;
 }
