@@ -41,7 +41,6 @@ struct LinRole {
   int reverse;                                                   // rows are visited from the last to the first
   int first_t;                                                   // `first` is read transposed
   int ws_t;                                                      // so are the segment states: they are another role's
-  int exact;                                                     // 16-bit operands: the state keeps all of its 32 bits
   int o32;                                                       // o is fp32 whatever the operands are
   float s_inter, s_state;                                        // factors of Y^T q and of k v^T (their product is the scale)
   const float* first;                                            // (B, H, HD, HD) state before the first row, or null
@@ -95,26 +94,35 @@ template <int NA, int NB> __device__ __forceinline__ f32x4 lin_mma(const lb8 (&a
   return c;
 }
 
-// A tile in LDS is its parts, each LIN_C rows of HD bf16 at a pitch of HD elements + 16 bytes.
+// A tile in LDS is its parts, each LIN_C rows of HD bf16.  Unit u (8 bytes) of row r lies at u ^ swz(r): 16 rows at one pair of units (row
+// reads), 8 rows x 4 units (transposed reads) and 256 bytes of neighbouring 16-byte pieces (writes) each cover the 64 banks once, and rows
+// 16 apart share it, so that a lane needs an address per unit and immediates for the rest.  (A padded pitch leaves 40 % of the LDS cycles
+// to conflicts: no pitch serves the row reads and the transposed ones.)
 template <typename T, int HD> struct LinTile {
-  static constexpr int IN = LinT<T>::IN, PITCH = 2 * HD + 16, PART = LIN_C * PITCH, BYTES = IN * PART;
+  static constexpr int IN = LinT<T>::IN, PITCH = 2 * HD, PART = LIN_C * PITCH, BYTES = IN * PART;
+  static __device__ __forceinline__ int swz(int r) {             // a permutation of the row bits that the pitch leaves on one bank, low ones on top
+    if (HD == 32) return (r & 4) | (r & 8) >> 2;                 // 4 rows to 256 bytes, 8 units to a row
+    if (HD == 64) return (r & 2) << 2 | (r & 4) | (r & 8) >> 2;
+    return (r & 1) << 4 | (r & 2) << 2 | (r & 4) | (r & 8) >> 2;
+  }
+  static __device__ __forceinline__ int at(int r, int u) { return r * PITCH + ((u ^ swz(r)) << 3); }
   static __device__ __forceinline__ void put(char* tile, int r, int c, lin_raw x) {            // 16 bytes, piece c of row r
-    if constexpr (IN == 1) *(lin_raw*)(tile + r * PITCH + 16 * c) = x;
+    if constexpr (IN == 1) *(lin_raw*)(tile + at(r, 2 * c)) = x;
     else {
       const f32x4 f = __builtin_bit_cast(f32x4, x);
       const float e[4] = {f[0], f[1], f[2], f[3]};
       unsigned w[IN][2];
       lin_split<IN, 2>(e, w);
 #pragma unroll
-      for (int k = 0; k < IN; ++k) *(lin_half*)(tile + k * PART + r * PITCH + 8 * c) = (lin_half){w[k][0], w[k][1]};
+      for (int k = 0; k < IN; ++k) *(lin_half*)(tile + k * PART + at(r, c)) = (lin_half){w[k][0], w[k][1]};
     }
   }
-  // 8 elements of row r at columns {32 kd + 4 g ..+3} and {32 kd + 16 + 4 g ..+3}: the order the state's accumulator tiles have
-  static __device__ __forceinline__ void row(const char* tile, int r, int kd, int g, lb8 (&f)[IN]) {
+  // 8 elements of row 16 rt + fr at columns {32 kd + 4 g ..+3} and {32 kd + 16 + 4 g ..+3}: the order the state's accumulator tiles have
+  static __device__ __forceinline__ void row(const char* tile, int rt, int fr, int kd, int g, lb8 (&f)[IN]) {
 #pragma unroll
     for (int k = 0; k < IN; ++k) {
-      const char* const p = tile + k * PART + r * PITCH + 64 * kd + 8 * g;
-      const lb4 a = *(const lb4*)p, b = *(const lb4*)(p + 32);
+      const char* const p = tile + k * PART + rt * 16 * PITCH;
+      const lb4 a = *(const lb4*)(p + at(fr, 8 * kd + g)), b = *(const lb4*)(p + at(fr, 8 * kd + 4 + g));
       f[k] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -122,7 +130,7 @@ template <typename T, int HD> struct LinTile {
   static __device__ __forceinline__ void col(const char* tile, int ct, int lane, lb8 (&f)[IN]) {
 #pragma unroll
     for (int k = 0; k < IN; ++k) {
-      const char* const p = tile + k * PART + (4 * (lane >> 4) + ((lane & 15) >> 2)) * PITCH + 32 * ct + 8 * (lane & 3);
+      const char* const p = tile + k * PART + at(4 * (lane >> 4) + ((lane & 15) >> 2), 4 * ct + (lane & 3));
       union { struct { s16x4 a, b; } s; lb8 v; } u;
       u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)p);
       u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)(p + 16 * PITCH));
@@ -173,11 +181,12 @@ __device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
-template <typename T, int HD, bool STATE>
+// EXACT: the state is a result (or might be: out does not depend on that) and keeps all of its 32 bits with a third part of the values.
+template <typename T, int HD, bool STATE, bool EXACT>
 __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
   typedef LinTile<T, HD> Tile;
-  constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = HD * (int)sizeof(T) + 16;       // OP: pitch of the result's tile, bytes
+  constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = Tile::IN == 1 ? 2 * HD : 4 * HD + 16;            // OP: pitch of the result's tile, bytes
   constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
   constexpr int WAVES = HD / 16, PP = 72, PPART = C * PP;        // scores: 32 rows of 32 bf16 at a pitch of 18 words (16 rows, 16 lanes: all banks)
@@ -315,7 +324,6 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
     w1[i] = scale * lin_pow(l2, 16 + d);
     wv[i] = r.s_state * lin_pow(l2, 16 - 4 * g - i);
   }
-  const bool exact = r.exact;
   const float l16 = lin_uniform(lin_pow(l2, 16)), lC = lin_uniform(lin_pow(l2, C)), lrow = r.s_inter * lin_pow(l2, fr);
 
   // one chunk of c rows; END: the segment's last one, which may be short and may end the sequence
@@ -327,6 +335,12 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
     f32x4 acc[2];                                                // results of the two query tiles
     acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if constexpr (!STATE) {
+      constexpr bool HOLD = L::IN == 1 && HD <= 64;              // else read again where they are used: too many registers
+      lb8 qf[2][NK][L::IN];
+      auto query = [&](int ti, int kd) __attribute__((always_inline)) { Tile::row(sQ, ti, fr, kd, g, qf[ti][kd]); };
+      if constexpr (HOLD)
+#pragma unroll
+        for (int kd = 0; kd < 2 * NK; ++kd) query(kd & 1, kd >> 1);
       // the scores of the tiles (queries, keys) = (0, 0), (1, 0), (1, 1), one wave to a tile, for all waves: in LDS, in parts
 #pragma unroll
       for (int n = 0; n < 3; ++n)
@@ -335,10 +349,10 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
           f32x4 p = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kd = 0; kd < NK; ++kd) {
-            lb8 qf[L::IN], kf[L::IN];
-            Tile::row(sQ, 16 * ti + fr, kd, g, qf);
-            Tile::row(sK, 16 * e + fr, kd, g, kf);
-            p = lin_mma(kf, qf, p);
+            lb8 kf[L::IN];
+            Tile::row(sK, e, fr, kd, g, kf);
+            if constexpr (!HOLD) query(ti, kd);
+            p = lin_mma(kf, qf[ti][kd], p);
           }
           float x[4];
 #pragma unroll
@@ -354,12 +368,11 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
-        lb8 y[L::MID], q0[L::IN], q1[L::IN];
+        lb8 y[L::MID];
         lin_split8<L::MID>(x, y);
-        Tile::row(sQ, fr, kd, g, q0);
-        Tile::row(sQ, 16 + fr, kd, g, q1);
-        acc[0] = lin_mma(y, q0, acc[0]);
-        acc[1] = lin_mma(y, q1, acc[1]);
+        if constexpr (!HOLD) { query(0, kd); query(1, kd); }
+        acc[0] = lin_mma(y, qf[0][kd], acc[0]);
+        acc[1] = lin_mma(y, qf[1][kd], acc[1]);
       }
       acc[0] *= lrow;
       acc[1] *= lrow * l16;
@@ -385,24 +398,14 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
           x[i] = j < c ? lin_value(vf, i) * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
         }
       }
-      // two parts of the weighted values; a state that leaves the call (or might: out does not depend on that) keeps its 32 bits with a third
-      lb8 p[3];
-      lin_split8<3>(x, p);
+      lb8 p[EXACT ? 3 : L::MID];
+      lin_split8<EXACT ? 3 : L::MID>(x, p);
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
-        lb8 kf[L::IN], m[L::MID];
-#pragma unroll
-        for (int i = 0; i < L::MID; ++i) m[i] = p[i];
+        lb8 kf[L::IN];
         Tile::col(sK, t, lane, kf);
-        S[t] = lin_mma(kf, m, S[t]);
+        S[t] = lin_mma(kf, p, S[t]);
       }
-      if (L::MID < 3 && exact)
-#pragma unroll
-        for (int t = 0; t < ND; ++t) {
-          lb8 kf[L::IN];
-          Tile::col(sK, t, lane, kf);
-          S[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[0], p[2], S[t], 0, 0, 0);
-        }
     }
     if constexpr (!STATE) {
       __syncthreads();
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
     if constexpr (!STATE) {
 #pragma unroll
       for (int ti = 0; ti < 2; ++ti) {
-        if (!o32) lin_store4((T*)(sO + (16 * ti + fr) * OP) + n0 + 4 * g, acc[ti]);
+        if (!o32) lin_store4((T*)(sO + (Tile::IN == 1 ? 16 * ti * OP + Tile::at(fr, n0 / 4 + g) : (16 * ti + fr) * OP + (n0 + 4 * g) * 4)), acc[ti]);
         else {
           const int t = t0 + 16 * ti + fr;
           if (t < upto) *(f32x4*)(out + n * r.o.n + (long long)(row0 + dir * t) * os + (n0 + 4 * g) * 4) = acc[ti];
@@ -440,7 +443,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           const int at = tid + u * THREADS;
-          if (!END || at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (at / CPR) * OP + (at % CPR) * 16), (lin_raw*)(bo + ao[u]));
+          if (!END || at / CPR < c) __builtin_nontemporal_store(*(const lin_raw*)(sO + (Tile::IN == 1 ? Tile::at(at / CPR, 2 * (at % CPR)) : (at / CPR) * OP + (at % CPR) * 16)), (lin_raw*)(bo + ao[u]));
         }
         bo += dO;
       }
@@ -619,20 +622,26 @@ static dim3 lin_grid(const LinArgs& a, int roles) {
   const unsigned groups = (unsigned)(((long long)a.slots * a.HK + 7) / 8);
   return dim3(8 * roles * a.rep, groups < LIN_GRID_Y ? groups : LIN_GRID_Y, (groups + LIN_GRID_Y - 1) / LIN_GRID_Y);
 }
-template <typename T, int HD>
+template <typename T, int HD, bool EXACT>
 static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
   const dim3 block(HD * 4);
   if (p.split) {
-    hipLaunchKernelGGL((lin_kernel<T, HD, true>), lin_grid(a, a.roles_state), block, 0, stream, a);
+    hipLaunchKernelGGL((lin_kernel<T, HD, true, EXACT>), lin_grid(a, a.roles_state), block, 0, stream, a);
     hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)((long long)a.H * HD * HD / 256 * a.B), a.roles_state), dim3(256), 0, stream, a, HD * HD);
   }
-  hipLaunchKernelGGL((lin_kernel<T, HD, false>), lin_grid(a, a.roles), block, 0, stream, a);
+  hipLaunchKernelGGL((lin_kernel<T, HD, false, EXACT>), lin_grid(a, a.roles), block, 0, stream, a);
 }
-template <typename T>
-static void lin_launch(const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {
-  if (HD == 32) lin_launch_hd<T, 32>(a, p, stream);
-  else if (HD == 64) lin_launch_hd<T, 64>(a, p, stream);
-  else lin_launch_hd<T, 128>(a, p, stream);
+template <typename T, bool EXACT>
+static void lin_launch_t(const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {
+  if (HD == 32) lin_launch_hd<T, 32, EXACT>(a, p, stream);
+  else if (HD == 64) lin_launch_hd<T, 64, EXACT>(a, p, stream);
+  else lin_launch_hd<T, 128, EXACT>(a, p, stream);
+}
+// exact: a state is a result, or might be
+static void lin_launch(int dtype, const LinArgs& a, const LinPlan& p, int HD, bool exact, hipStream_t stream) {
+  if (dtype == A2V_F32) lin_launch_t<float, false>(a, p, HD, stream);        // (three parts of everything as it is)
+  else if (exact) lin_launch_t<__bf16, true>(a, p, HD, stream);
+  else lin_launch_t<__bf16, false>(a, p, HD, stream);
 }
 static int lin_dtype(int dtype) {
   if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
@@ -671,11 +680,10 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
   lin_args(a, p, slopes, cu_seqlens, B, S, H, HK, zero_outside);
   const int kv = H != HK ? 6 : 0;
   a.r[0] = LinRole{lin_op(q, strides, es), lin_op(k, strides + 3, es), lin_op(v, strides + 6, es), lin_op(out, strides + 9, es),
-                   kv, 0, 0, 0, 1, 0, scale, 1.f, state, state_out, (float*)ws};
+                   kv, 0, 0, 0, 0, scale, 1.f, state, state_out, (float*)ws};
   a.r[1] = a.r[2] = a.r[0];
   a.roles = a.roles_state = 1;
-  if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
-  else lin_launch<__bf16>(a, p, HD, stream);
+  lin_launch(dtype, a, p, HD, true, stream);
   A2V_CHECK_LAUNCH();
   return A2V_OK;
 }
@@ -710,12 +718,11 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
     gv = lin_op(dv32, one, 4);
   }
   const int o32 = rep > 1, kv = rep > 1;
-  a.r[0] = LinRole{D, V, K, o[4], 6 * kv, 0, 1, 0, 0, 0, scale, 1.f, state, nullptr, (float*)w};
-  a.r[1] = LinRole{K, Q, D, gv, kv, 1, 0, 0, d_state != nullptr, o32, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
-  a.r[2] = LinRole{V, D, Q, gk, kv, 1, 1, 1, 0, o32, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
+  a.r[0] = LinRole{D, V, K, o[4], 6 * kv, 0, 1, 0, 0, scale, 1.f, state, nullptr, (float*)w};
+  a.r[1] = LinRole{K, Q, D, gv, kv, 1, 0, 0, o32, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
+  a.r[2] = LinRole{V, D, Q, gk, kv, 1, 1, 1, o32, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
   a.roles = 3; a.roles_state = 2;                                // dk's segment states are the transposes of dv's
-  if (dtype == A2V_F32) lin_launch<float>(a, p, HD, stream);
-  else lin_launch<__bf16>(a, p, HD, stream);
+  lin_launch(dtype, a, p, HD, d_state != nullptr, stream);
   if (rep > 1 && rows) {
     const dim3 grid((unsigned)cdiv((long)(rows * HK * HD / 4), 256));
     if (dtype == A2V_F32)
