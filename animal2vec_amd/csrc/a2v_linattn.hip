@@ -63,7 +63,9 @@ struct LinArgs {
 // segments: 16 heads x 64 x 16 KB for each of them).  One clip of 16 segments: 23.0 us with the scan kernel, 17.8 without.
 #define LIN_INLINE 16
 
-#define LIN_C 32              /* rows of a chunk: two tiles of 16 */
+#define LIN_C 32              /* rows of a chunk: two tiles of 16.  64 rows pay the state's share half as often and meet half the barriers, but
+                                 take 168 registers in place of 128: 3 workgroups on a CU, not 4 (512 x 2000 rows: 248 us against 223; the
+                                 training pair 208 against 168) */
 template <typename T> struct LinT;
 template <> struct LinT<__bf16> { static constexpr int IN = 1, MID = 2, V = 8; };      // parts of the operands, of scores and states; elements of 16 bytes
 template <> struct LinT<float> { static constexpr int IN = 3, MID = 3, V = 4; };
