@@ -12,8 +12,9 @@
 // so ONE kernel does all four: a "role" names its operands, its direction and where the scale goes.
 //
 // One workgroup owns a (sequence, head) or a segment of one and walks its chunks with the state in registers.  A wave owns 16 columns
-// of v: the whole HD x 16 slice of the state lives in its MFMA accumulators, whose layout IS the A operand of Y^T q, so neither the
-// state nor the scores ever pass through LDS; the price is that every wave forms the chunk's scores itself.
+// of v: the whole HD x 16 slice of the state lives in its MFMA accumulators, whose layout IS the A operand of Y^T q, so the state never
+// passes through LDS.  The scores do: a wave forms one 16 x 16 tile of them for all waves (each wave forming all of them instead: 183 us
+// against 173 for the training pair of 152-row clips, 323 against 285 with 128 channels).
 // Products are issued swapped (P^T = K Q^T, O^T = V^T P^T + Y^T Q^T): see a2v_attn.hip for the layout argument.
 //
 // All products run on the bf16 matrix cores, fp32 values as sums of bf16 parts of 8 bits each (x = hi + mid + lo exactly; the products of
@@ -625,7 +626,7 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
   if (rows >= (1LL << 30)) return false;
   p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
   const long long slots = packed ? (long long)S / p.seg + B + 1 : (long long)B * (S > p.seg ? (S + p.seg - 1) / p.seg : 1);
-  if ((slots + 8) * H * 3 >= (1LL << 31) || (long long)B * H * HD * HD / 256 >= (1LL << 31)) return false;
+  if ((slots + 8) * H * 3 >= (1LL << 31) || (long long)B * H * HD * HD >= (1LL << 32)) return false;       // (a launch has at most 2^32 threads in x)
   p.slots = (int)slots;
   p.split = S > p.seg;
   p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
@@ -633,6 +634,11 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
 }
 static bool lin_shape_ok(int B, int S, int H, int HK, int HD) {
   return B >= 0 && S >= 0 && H > 0 && HK > 0 && H % HK == 0 && H / HK <= 1024 && (HD == 32 || HD == 64 || HD == 128);
+}
+// The state that a call leaves may not lie in the one that it reads: every segment of a sequence starts from the latter.
+static bool lin_states_apart(const float* in, const float* out, int B, int H, int HD) {
+  const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out, n = (uintptr_t)B * H * HD * HD * sizeof(float);
+  return !in || !out || a + n <= b || b + n <= a;
 }
 static bool lin_tensor_ok(const void* p, const long long* st, int es) {
   return p && !((uintptr_t)p & 15) && !((st[0] * es) & 15) && !((st[1] * es) & 15) && !((st[2] * es) & 15) && st[1] >= 0 &&
@@ -696,6 +702,7 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
   const int es = dtype == A2V_F32 ? 4 : 2;
   if (S > 0 && !(lin_tensor_ok(q, strides, es) && lin_tensor_ok(k, strides + 3, es) && lin_tensor_ok(v, strides + 6, es) && lin_tensor_ok(out, strides + 9, es)))
     return A2V_ERR_ARG;
+  if (!lin_states_apart(state, state_out, B, H, HD)) return A2V_ERR_ARG;
   if (p.states > ws_bytes || (p.states && (!ws || ((uintptr_t)ws & 15)))) return A2V_ERR_ARG;
   LinArgs a;
   lin_args(a, p, slopes, cu_seqlens, B, S, H, HK, zero_outside);
@@ -722,6 +729,8 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
   if (S > 0)
     for (int i = 0; i < 7; ++i)
       if (!lin_tensor_ok(t[i], strides + 3 * i, es)) return A2V_ERR_ARG;
+  if (!lin_states_apart(state, d_state, B, H, HD) || !lin_states_apart(d_state_out, d_state, B, H, HD)) return A2V_ERR_ARG;
+  if (rep > 1 && (cu_seqlens ? 1LL : (long long)B) * S * HK * HD / 4 >= (1LL << 32)) return A2V_ERR_ARG;    // (threads of the join)
   const size_t need = a2v_linear_attention_workspace(dtype, 1, cu_seqlens != nullptr, B, S, H, HK, HD);
   if (need > ws_bytes || (need && (!ws || ((uintptr_t)ws & 15)))) return A2V_ERR_ARG;
   char* w = (char*)ws;
@@ -762,7 +771,7 @@ extern "C" int a2v_linear_attention_step(int dtype, const void* q, const void* k
                                          hipStream_t stream) {
   if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
   if (!strides || !slopes || !state || ((uintptr_t)state & 15) || N < 0 || H <= 0 || HK <= 0 || H % HK || (HD != 32 && HD != 64 && HD != 128) ||
-      n_slots < (slots ? 0 : N) || (long long)N * H >= (1LL << 31))
+      n_slots < (slots ? 0 : N) || (long long)N * H >= (1LL << 24))              // (2^32 threads)
     return A2V_ERR_ARG;
   if (N == 0) return A2V_OK;
   const int es = dtype == A2V_F32 ? 4 : 2;

@@ -272,7 +272,7 @@ extern "C" int a2v_qk_norm_rope_fwd(int dtype, const void* q, const void* k, voi
   a.t[1] = QknOne{k, nullptr, k_out, s[3], s[4], s[5], 0, 0, 0, s[9], s[10], s[11], k_weight, HK};
   a.rows = qkn_rows(a.M, H + HK, HD);
   const long long blocks = (a.M + a.rows - 1) / a.rows;
-  if (blocks >= (1LL << 31)) return A2V_ERR_ARG;
+  if (blocks >= (1LL << 24)) return A2V_ERR_ARG;                  // (2^32 threads)
   QKN_LAUNCH(qkn_fwd_kernel, dim3((unsigned)blocks));
   A2V_CHECK_LAUNCH();
   return A2V_OK;

@@ -622,8 +622,12 @@ def _heads(what, t, dims, like=None, out=False):
         raise ValueError(f"{what}: the channels of a head must be contiguous and every head start on 16 bytes, got strides {st}")
     if dims == 4 and t.shape[1] > 1 and st[1] * t.element_size() >= 1 << 26:
         raise ValueError(f"{what}: rows {st[1]} elements apart (most: 64 MiB)")
-    if out and any(s < t.shape[-1] for s, n in zip(st[:-1], t.shape) if n > 1):
-        raise ValueError(f"{what}: an output may not repeat memory, got strides {st}")
+    if out:
+        reach = t.shape[-1]                                      # elements that the dimensions of smaller strides cover
+        for s, n in sorted((s, n) for s, n in zip(st[:-1], t.shape) if n > 1):
+            if s < reach:
+                raise ValueError(f"{what}: an output may not repeat memory, got shape {tuple(t.shape)}, strides {st}")
+            reach += (n - 1) * s
 
 
 def _results(what, named, out=True):
@@ -660,12 +664,12 @@ def _overlap(a, b):
     return d < wide[1] or min(rows) - d < wide[0]
 
 
-def _apart(what, outs, ins, inplace=()):
-    """no output shares memory with an input or another output; output i may be inplace[i] itself"""
+def _apart(what, outs, ins, inplace=False):
+    """no output shares memory with an input or another output; inplace: output i may be input i itself (no other input, not even if the
+    same tensor was given for both)"""
     for i, o in enumerate(outs):
-        for t in ins:
-            me = inplace[i] if i < len(inplace) else None
-            if t is me and o.data_ptr() == t.data_ptr() and all(x == y or n == 1 for x, y, n in zip(o.stride(), t.stride(), o.shape)):
+        for j, t in enumerate(ins):
+            if inplace and i == j and o.data_ptr() == t.data_ptr() and all(x == y or n == 1 for x, y, n in zip(o.stride(), t.stride(), o.shape)):
                 continue
             if _overlap(o, t):
                 raise ValueError(f"{what}: an output overlaps an input")
@@ -728,13 +732,13 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, inv_freq, pos=None, *, sections=N
         p = _qk_norm_rope_checks(what, q, k, q_weight, k_weight, inv_freq, pos, sections)
         _results(what, (("q_out", q_out, q), ("k_out", k_out, k)))
         if given:
-            _apart(what, (q_out, k_out), (q, k), (q, k))         # (before the device check: a refusal does not depend on the device)
+            _apart(what, (q_out, k_out), (q, k), inplace=True)         # (before the device check: a refusal does not depend on the device)
         _starts(what, q, k, q_out, k_out, q_weight, k_weight)
         _on_gpu(q)
         return (_strides(q, k, q_out, k_out), *p)
     st, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections), (q, k, q_weight, k_weight, inv_freq, pos, *((q_out, k_out) if given else ())), plan)
     if given:
-        _apart(what, (q_out, k_out), (q, k), (q, k))
+        _apart(what, (q_out, k_out), (q, k), inplace=True)
     if q.numel() == 0:
         return q_out, k_out
     _run(_L().a2v_qk_norm_rope_fwd, "a2v_qk_norm_rope_fwd", q.device, code, *_starts(what, q, k, q_out, k_out), st, *_starts(what, q_weight, k_weight),
@@ -759,17 +763,19 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, inv_freq, pos=Non
         _results(what, (("dq", dq, q), ("dk", dk, k)))
         _f32(f"{what}: dq_weight", dq_weight, (q.shape[3],), q)
         _f32(f"{what}: dk_weight", dk_weight, (q.shape[3],), q)
-        if dq_weight.data_ptr() == dk_weight.data_ptr():
+        if abs(dq_weight.data_ptr() - dk_weight.data_ptr()) < 4 * q.shape[3]:
             raise ValueError(f"{what}: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
+        if given:
+            _apart(what, (dq, dk), (dq_out, dk_out, q, k), inplace=True)
         _starts(what, dq_out, dk_out, q, k, dq, dk, q_weight, k_weight)
         _on_gpu(q)
         return (_strides(dq_out, dk_out, q, k, dq, dk), _L().a2v_qk_norm_rope_workspace(*p[-1]), *p)
     st, need, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections),
                                                    (q, k, q_weight, k_weight, inv_freq, pos, dq_out, dk_out, dq_weight, dk_weight, *((dq, dk) if given else ())), plan)
-    if dq_weight.data_ptr() == dk_weight.data_ptr():
+    if abs(dq_weight.data_ptr() - dk_weight.data_ptr()) < 4 * q.shape[3]:
         raise ValueError(f"{what}: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
     if given:
-        _apart(what, (dq, dk), (dq_out, dk_out, q, k), (dq_out, dk_out))
+        _apart(what, (dq, dk), (dq_out, dk_out, q, k), inplace=True)
     if q.numel() == 0:
         return dq, dk
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)

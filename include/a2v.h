@@ -209,17 +209,19 @@ int a2v_qk_norm_rope_bwd(int dtype, const void* dq_out, const void* dk_out, cons
 size_t a2v_qk_norm_rope_workspace(int N, int S, int H, int HK, int HD);
 /* S_t = exp(-slopes[h]) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t;  slopes (H) fp32, >= 0 (infinity: only the row itself).
  * state / state_out (B, H, HD, HD) fp32 [channel of k][channel of v], before the first and behind the last row, either may be NULL;
- * both may be the same buffer.
+ * they may not overlap (every part of a long sequence starts from the former).
  * cu_seqlens NULL: B sequences of S rows.  Else the tensors have S rows (sequence strides unused), sequence b is rows
  * cu_seqlens[b] .. cu_seqlens[b + 1] (B + 1 int32 on the device, ascending; a sequence may be empty: its state is handed on).  Rows
  * outside every sequence are left alone, or set to 0 with zero_outside.  Offsets outside [0, S] are clamped.
  * ws: a2v_linear_attention_workspace() bytes (0 where the axis is not split), 16-byte aligned; used by this call only.
  * dtype A2V_F32 or A2V_BF16; liba2v_hip_f16.so refuses its 16-bit type (A2V_ERR_UNSUPPORTED: a state does not fit half's range).
- * A non-finite value reaches the rows of its own 64-row block and those behind it, never another sequence. */
+ * A non-finite value reaches the rows of its own 32-row block and those behind it (gradients of k and v: in
+ * front of it), never another sequence.
+ * Limits, else A2V_ERR_ARG: fewer than 2^30 rows, rows less than 64 MiB apart, H / HK <= 1024, B H HD HD < 2^32. */
 int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, const float* slopes,
                              const float* state, float* state_out, const int* cu_seqlens, int B, int S, int H, int HK, int HD, float scale,
                              int zero_outside, void* ws, size_t ws_bytes, a2v_stream_t stream);
-/* d_state_out: gradient of state_out or NULL; d_state: gradient of state or NULL.  No atomics: the same call gives the same bits. */
+/* d_state_out: gradient of state_out or NULL; d_state: gradient of state or NULL, apart from state and d_state_out.  No atomics: the same call gives the same bits. */
 int a2v_linear_attention_bwd(int dtype, const void* q, const void* k, const void* v, const void* d_out, void* dq, void* dk, void* dv,
                              const long long* strides, const float* slopes, const float* state, const float* d_state_out, float* d_state,
                              const int* cu_seqlens, int B, int S, int H, int HK, int HD, float scale, int zero_outside, void* ws,

@@ -161,9 +161,19 @@ def test_outputs_may_not_overlap():
     for go in (lambda: ops.qk_norm_rope_fwd(**rope, q_out=q, k_out=k), lambda: ops.linear_attention_fwd(q, k, v, slopes, out=torch.zeros_like(d))):
         with pytest.raises(_lib.A2VError):
             go()
-    w = torch.zeros(64)
-    with pytest.raises(ValueError, match="two buffers"):
-        ops.qk_norm_rope_bwd(d, d, **dict(a, q=d, k=d), dq_weight=w, dk_weight=w)
+    w = torch.zeros(96)
+    for dk_weight in (w[:64], w[32:]):
+        with pytest.raises(ValueError, match="two buffers"):
+            ops.qk_norm_rope_bwd(d, d, **dict(a, q=d, k=d), dq_weight=w[:64], dk_weight=dk_weight)
+    # one tensor given twice: in place for q would change k under its reader
+    with pytest.raises(ValueError, match="overlap"):
+        ops.qk_norm_rope_fwd(**dict(a, q=q, k=q), q_out=q)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.qk_norm_rope_bwd(d, d, **dict(a, q=q, k=k), dq_weight=w[:64], dk_weight=torch.zeros(64), dq=d)
+    # rows and heads of an output that meet
+    for strides in ((1280, 64, 64, 1), (1280, 128, 64, 1), (256, 256, 64, 1)):
+        with pytest.raises(ValueError, match="repeat"):
+            ops.linear_attention_fwd(d, d, d, slopes, out=torch.zeros(2 * 1280 * 4, dtype=torch.bfloat16).as_strided((2, 5, 4, 64), strides))
 
 
 def _lin_args(N=2, S=5, H=4, HK=2, HD=64, dtype=torch.bfloat16):
@@ -221,12 +231,20 @@ def test_c_entries_refuse_bad_arguments():
         assert fwd(dtype=7) == -2 and fwd(q=None) == -1 and fwd(o=p + 4) == -1 and fwd(st=None) == -1 and fwd(sl=None) == -1 and fwd(H=3) == -1 and fwd(HD=48) == -1
         assert fwd(st=(C.c_longlong * 12)(*([66] * 12))) == -1 and fwd(B=0) == 0 and fwd(B=-1) == -1 and fwd(S=1 << 30) == -1
         assert fwd(B=1, S=100000) == -1                            # no workspace
+        assert fwd(B=1 << 20, S=1, H=4096, HK=4096) == -1          # 2^32 elements of state
+        # a state that is left where one is read
+        n = 2 * 64 * 64 * 4
+        for first, last in ((p, p), (p, p + n - 16), (p + n - 16, p)):
+            assert lib.a2v_linear_attention_fwd(0, p, p, p, p, st, p, first, last, None, 1, 4, 2, 2, 64, 1.0, 0, None, 0, None) == -1
+            assert lib.a2v_linear_attention_bwd(0, p, p, p, p, p, p, p, st, p, first, None, last, None, 1, 4, 2, 2, 64, 1.0, 0, None, 0, None) == -1
+            assert lib.a2v_linear_attention_bwd(0, p, p, p, p, p, p, p, st, p, None, first, last, None, 1, 4, 2, 2, 64, 1.0, 0, None, 0, None) == -1
         assert fwd(dtype=1, B=0) == (-4 if half else 0)
         need = lib.a2v_linear_attention_workspace(0, 1, 0, 1, 100000, 2, 1, 64)
         assert need > 2 * 100000 * 2 * 64 * 4 and lib.a2v_linear_attention_workspace(0, 0, 0, 64, 2000, 16, 16, 64) == 0
         assert lib.a2v_linear_attention_bwd(0, p, p, p, p, p, p, p, st, p, None, None, None, None, 1, 100000, 2, 1, 64, 1.0, 0, p, need - 1, None) == -1
         assert lib.a2v_linear_attention_step(0, p, p, p, p, st, p, None, None, 4, 4, 2, 2, 64, 1.0, None) == -1
         assert lib.a2v_linear_attention_step(0, p, p, p, p, st, p, p, None, 3, 4, 2, 2, 64, 1.0, None) == -1
+        assert lib.a2v_linear_attention_step(0, p, p, p, p, st, p, p, p, 1, 1 << 23, 2, 2, 64, 1.0, None) == -1
         assert lib.a2v_linear_attention_step(0, p + 4, p, p, p, st, p, p, p, 3, 4, 2, 2, 64, 1.0, None) == -1
 
         def rope(dtype=0, q=p, w=p, f=p, pos=p, ps=(C.c_longlong * 2)(4, 1), axes=3, sec=sec, HD=64, N=1):
@@ -646,12 +664,12 @@ def test_streams_and_captured_graphs(ops):
 @gpu
 def test_long_offsets_pass_32_bits(ops):
     """a packed buffer of more than 2^31 elements: the last rows are as right as the first ones (addresses are formed in 64 bits)"""
-    H, HD, W = 2, 64, 3 * 16 * 64
-    S = 700032                                                   # S * W = 2.15e9 elements
+    H, HD, W = 2, 64, 60 * 64
+    S = 560032                                                   # S * W = 2.15e9 elements
     base = torch.empty(S, W, dtype=torch.bfloat16, device="cuda")
-    view = base.view(1, S, 48, HD)
+    view = base.view(1, S, 60, HD)
     assert base.numel() > 2 ** 31
-    q, k, v = view[:, :, 0:H], view[:, :, 16:16 + H], view[:, :, 46:46 + H]
+    q, k, v = view[:, :, 0:H], view[:, :, 20:20 + H], view[:, :, 58:58 + H]
     for i, t in enumerate((q, k, v)):
         t.copy_(torch.randn(1, S, H, HD, generator=torch.Generator("cuda").manual_seed(i), device="cuda").to(torch.bfloat16))
     sl = torch.tensor([0.5, 1.0], device="cuda")
