@@ -189,7 +189,7 @@ __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amd
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 // EXACT: the state is a result (or might be: out does not depend on that) and keeps all of its 32 bits with a third part of the values.
 template <typename T, int HD, bool STATE, bool EXACT>
-__global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(LinArgs a) {
+__global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
   typedef LinTile<T, HD> Tile;
   constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = Tile::IN == 1 ? 2 * HD : 4 * HD + 16;            // OP: pitch of the result's tile, bytes
@@ -204,7 +204,10 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
   char* const sP = sO + (STATE ? 0 : C * OP);
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
-  const int nr = STATE ? a.roles_state : a.roles, in = blockIdx.x >> 3, unit = (blockIdx.z * LIN_GRID_Y + blockIdx.y) * 8 + (blockIdx.x & 7);
+  const int nr = STATE ? a.roles_state : a.roles, in = blockIdx.x >> 3, turn = blockIdx.z * LIN_GRID_Y + blockIdx.y;
+  // Neighbouring heads go to neighbouring XCDs, except where two of them share a cache line (32 channels of 16 bits: 320 us one by one, 293
+  // in pairs for 64 x 2000 rows of 32 heads; pairs of 64 channels: 230 against 225).
+  const int unit = HD * (int)sizeof(T) < 128 ? (turn >> 1) * 16 + (blockIdx.x & 7) * 2 + (turn & 1) : turn * 8 + (blockIdx.x & 7);
   const int of = nr == 1 ? in : nr == 2 ? in >> 1 : in * 21846 >> 16;         // in / nr (in < 3 * 4096)
   const int slot0 = unit / a.HK, hk = unit - slot0 * a.HK, h = hk * a.rep + of;
   if (slot0 >= a.slots) return;
@@ -489,33 +492,31 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN > 1 ? 2 : 4) void lin_kernel(Li
 
 // ws[slot] := the state in front of segment p from the segments before it: carried through the sequence's slots in order, one thread to an
 // element (any order of them: the waves' register image), eight loads in flight.  The part of `first` is added by the kernel that starts
-// from it.
+// from it.  At most LIN_SCANS sequences are in work at a time: short ones of a packed batch, which have nothing to scan, cost a look each
+// (37 of them with a workgroup apiece: 4.7 us).
+#define LIN_SCANS 8
 __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
-  const int per = a.H * HH / 256, b = blockIdx.x / per;
-  LinSeq s;
-  if (a.cu) {
-    s.begin = lin_cu(a, b);
-    const int end = lin_cu(a, b + 1);
-    s.len = end > s.begin ? end - s.begin : 0;
-  } else { s.begin = 0; s.len = a.S; }
-  s.np = s.len > a.seg ? (s.len + a.seg - 1) / a.seg : 1;
-  if (s.np <= LIN_INLINE) return;
-  const int slot0 = a.cu ? s.begin / a.seg + b : b * s.np;
-  const int i = (blockIdx.x - b * per) * 256 + threadIdx.x, h = i / HH;        // element of (H, HD, HD); HD * HD % 256 == 0
+  const int per = a.H * HH / 256, b0 = blockIdx.x / per;
+  const int i = (blockIdx.x - b0 * per) * 256 + threadIdx.x, h = i / HH;       // element of (H, HD, HD); HD * HD % 256 == 0
   const float f = lin_pow(lin_log2(a.slopes, h), a.seg);
   const long long step = (long long)a.H * HH;
-  float* const w = a.r[blockIdx.y].ws + slot0 * step + i;
-  float carry = 0.f;
-  int p = 0;
-  for (; p + 8 < s.np; p += 8) {                                 // (the last segment has no state of its own)
-    float x[8];
+  for (int b = b0; b < a.B; b += LIN_SCANS) {
+    const int begin = a.cu ? lin_cu(a, b) : 0, len = a.cu ? lin_cu(a, b + 1) - begin : a.S;
+    const int np = len > a.seg ? (len + a.seg - 1) / a.seg : 1;
+    if (np <= LIN_INLINE) continue;
+    float* const w = a.r[blockIdx.y].ws + (long long)(a.cu ? begin / a.seg + b : b * np) * step + i;
+    float carry = 0.f;
+    int p = 0;
+    for (; p + 8 < np; p += 8) {                                 // (the last segment has no state of its own)
+      float x[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) x[u] = w[(p + u) * step];
+      for (int u = 0; u < 8; ++u) x[u] = w[(p + u) * step];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) { w[(p + u) * step] = carry; carry = carry * f + x[u]; }
+      for (int u = 0; u < 8; ++u) { w[(p + u) * step] = carry; carry = carry * f + x[u]; }
+    }
+    for (; p < np - 1; ++p) { const float x = w[p * step]; w[p * step] = carry; carry = carry * f + x; }
+    w[p * step] = carry;
   }
-  for (; p < s.np - 1; ++p) { const float x = w[p * step]; w[p * step] = carry; carry = carry * f + x; }
-  w[p * step] = carry;
 }
 
 // the gradients of a shared k / v head: the sum over its heads, of fp32 rows (T, H, HD) -> rows of HK heads
@@ -626,7 +627,7 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
   if (rows >= (1LL << 30)) return false;
   p.seg = lin_seg(B, rows, S, H, HD, packed, p.C);
   const long long slots = packed ? (long long)S / p.seg + B + 1 : (long long)B * (S > p.seg ? (S + p.seg - 1) / p.seg : 1);
-  if ((slots + 8) * H * 3 >= (1LL << 31) || (long long)B * H * HD * HD >= (1LL << 32)) return false;       // (a launch has at most 2^32 threads in x)
+  if ((slots + 16) * H * 3 >= (1LL << 31) || (long long)H * HD * HD >= (1LL << 28)) return false;      // (a launch has at most 2^32 threads in x)
   p.slots = (int)slots;
   p.split = S > p.seg;
   p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
@@ -646,7 +647,7 @@ static bool lin_tensor_ok(const void* p, const long long* st, int es) {
 }
 
 static dim3 lin_grid(const LinArgs& a, int roles) {
-  const unsigned groups = (unsigned)(((long long)a.slots * a.HK + 7) / 8);
+  const unsigned groups = (unsigned)(((long long)a.slots * a.HK + 15) / 16 * 2);       // (of eight, in pairs)
   return dim3(8 * roles * a.rep, groups < LIN_GRID_Y ? groups : LIN_GRID_Y, (groups + LIN_GRID_Y - 1) / LIN_GRID_Y);
 }
 template <typename T, int HD, bool EXACT>
@@ -654,7 +655,7 @@ static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream
   const dim3 block(HD * 4);
   if (p.split) {
     hipLaunchKernelGGL((lin_kernel<T, HD, true, EXACT>), lin_grid(a, a.roles_state), block, 0, stream, a);
-    if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)((long long)a.H * HD * HD / 256 * a.B), a.roles_state), dim3(256), 0, stream, a, HD * HD);
+    if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)a.H * (HD * HD / 256) * (a.B < LIN_SCANS ? a.B : LIN_SCANS), a.roles_state), dim3(256), 0, stream, a, HD * HD);
   }
   hipLaunchKernelGGL((lin_kernel<T, HD, false, EXACT>), lin_grid(a, a.roles), block, 0, stream, a);
 }

@@ -217,7 +217,8 @@ size_t a2v_qk_norm_rope_workspace(int N, int S, int H, int HK, int HD);
  * dtype A2V_F32 or A2V_BF16; liba2v_hip_f16.so refuses its 16-bit type (A2V_ERR_UNSUPPORTED: a state does not fit half's range).
  * A non-finite value reaches the rows of its own 32-row block and those behind it (gradients of k and v: in
  * front of it), never another sequence.
- * Limits, else A2V_ERR_ARG: fewer than 2^30 rows, rows less than 64 MiB apart, H / HK <= 1024, B H HD HD < 2^32. */
+ * Limits, else A2V_ERR_ARG: fewer than 2^30 rows, rows less than 64 MiB apart, H / HK <= 1024, H HD HD < 2^28, fewer
+ * than 2^31 / 3 / H segments. */
 int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, const float* slopes,
                              const float* state, float* state_out, const int* cu_seqlens, int B, int S, int H, int HK, int HD, float scale,
                              int zero_outside, void* ws, size_t ws_bytes, a2v_stream_t stream);

@@ -231,7 +231,7 @@ def test_c_entries_refuse_bad_arguments():
         assert fwd(dtype=7) == -2 and fwd(q=None) == -1 and fwd(o=p + 4) == -1 and fwd(st=None) == -1 and fwd(sl=None) == -1 and fwd(H=3) == -1 and fwd(HD=48) == -1
         assert fwd(st=(C.c_longlong * 12)(*([66] * 12))) == -1 and fwd(B=0) == 0 and fwd(B=-1) == -1 and fwd(S=1 << 30) == -1
         assert fwd(B=1, S=100000) == -1                            # no workspace
-        assert fwd(B=1 << 20, S=1, H=4096, HK=4096) == -1          # 2^32 elements of state
+        assert fwd(B=1, S=1, H=1 << 16, HK=1 << 16) == -1          # 2^28 elements of state in one sequence
         # a state that is left where one is read
         n = 2 * 64 * 64 * 4
         for first, last in ((p, p), (p, p + n - 16), (p + n - 16, p)):
