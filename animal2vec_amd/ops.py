@@ -572,7 +572,13 @@ _LAYOUTS = {}
 
 
 def _layout(name, opts, ts, make):
-    key = (name, _HALF, opts, *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in ts])
+    key = [name, _HALF, opts]
+    for t in ts:
+        if t is None:
+            key.append(None)
+        else:
+            key += (t.shape, t.stride(), t.dtype, t.get_device())
+    key = tuple(key)
     p = _LAYOUTS.get(key)
     if p is None:
         p = make()
@@ -584,25 +590,29 @@ def _layout(name, opts, ts, make):
 
 def _run(fn, what, device, *args):
     """fn(*args, stream) on the current stream of `device`, which need not be the current device"""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(device.index))
+    index = device.index
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device.index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, what)
 
 
-# the handle without a Stream object around it, where this torch has it (1 us a call)
+# the device and the stream's handle without Python objects around them, where this torch has that (1 us a call)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _starts(what, *ts):
     """data pointers, on 16 bytes each"""
     ps = [t.data_ptr() for t in ts]
+    low = 0
     for p in ps:
-        if p & 15:
-            raise ValueError(f"{what}: every tensor of heads must start on 16 bytes")
+        low |= p
+    if low & 15:
+        raise ValueError(f"{what}: every tensor of heads must start on 16 bytes")
     return ps
 
 
