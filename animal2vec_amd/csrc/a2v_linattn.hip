@@ -100,18 +100,21 @@ template <int NA, int NB> __device__ __forceinline__ f32x4 lin_mma(const lb8 (&a
   return c;
 }
 
-// A tile in LDS is its parts, each LIN_C rows of HD bf16.  Unit u (8 bytes) of row r lies at u ^ swz(r): 16 rows at one pair of units (row
-// reads), 8 rows x 4 units (transposed reads) and 256 bytes of neighbouring 16-byte pieces (writes) each cover the 64 banks once, and rows
-// 16 apart share it, so that a lane needs an address per unit and immediates for the rest.  (A padded pitch leaves 40 % of the LDS cycles
-// to conflicts: no pitch serves the row reads and the transposed ones.)
+// A tile in LDS is its parts, each LIN_C rows of HD bf16.  Piece p (16 bytes) of row r lies at p ^ swz(r): 16 rows at one piece (row reads) and
+// 256 bytes of neighbouring pieces (writes) each cover the 64 banks once, the transposed reads of half pieces twice, and rows 16 apart share
+// it, so that a lane needs an address per piece and immediates for the rest.  (A padded pitch leaves 40 % of the LDS cycles to conflicts: no
+// pitch serves the row reads and the transposed ones.)
+//
+// Channel 32 kd + 8 g + 4 h + i is row 4 g + i of the state's tile 2 kd + h, so that the eight channels which a lane group g holds of a pair of
+// tiles -- the inner index of Y^T q -- are one piece of a row of q.
 template <typename T, int HD> struct LinTile {
   static constexpr int IN = LinT<T>::IN, PITCH = 2 * HD, PART = LIN_C * PITCH, BYTES = IN * PART;
-  static __device__ __forceinline__ int swz(int r) {             // a permutation of the row bits that the pitch leaves on one bank, low ones on top
-    if (HD == 32) return (r & 4) | (r & 8) >> 2;                 // 4 rows to 256 bytes, 8 units to a row
-    if (HD == 64) return (r & 2) << 2 | (r & 4) | (r & 8) >> 2;
-    return (r & 1) << 4 | (r & 2) << 2 | (r & 4) | (r & 8) >> 2;
+  static __device__ __forceinline__ int swz(int r) {             // the row bits that the pitch leaves on one bank, reversed
+    if (HD == 32) return (r & 4) >> 1 | (r & 8) >> 3;            // 4 rows to 256 bytes, 4 pieces to a row
+    if (HD == 64) return (r & 2) << 1 | (r & 4) >> 1 | (r & 8) >> 3;
+    return (r & 1) << 3 | (r & 2) << 1 | (r & 4) >> 1 | (r & 8) >> 3;
   }
-  static __device__ __forceinline__ int at(int r, int u) { return r * PITCH + ((u ^ swz(r)) << 3); }
+  static __device__ __forceinline__ int at(int r, int u) { return r * PITCH + (((u >> 1) ^ swz(r)) << 4) + ((u & 1) << 3); }     // u: half pieces
   static __device__ __forceinline__ void put(char* tile, int r, int c, lin_raw x) {            // 16 bytes, piece c of row r
     if constexpr (IN == 1) *(lin_raw*)(tile + at(r, 2 * c)) = x;
     else {
@@ -123,27 +126,26 @@ template <typename T, int HD> struct LinTile {
       for (int k = 0; k < IN; ++k) *(lin_half*)(tile + k * PART + at(r, c)) = (lin_half){w[k][0], w[k][1]};
     }
   }
-  // 8 elements of row 16 rt + fr at columns {32 kd + 4 g ..+3} and {32 kd + 16 + 4 g ..+3}: the order the state's accumulator tiles have
+  // 8 elements of row 16 rt + fr at columns 32 kd + 8 g ..+7
   static __device__ __forceinline__ void row(const char* tile, int rt, int fr, int kd, int g, lb8 (&f)[IN]) {
 #pragma unroll
-    for (int k = 0; k < IN; ++k) {
-      const char* const p = tile + k * PART + rt * 16 * PITCH;
-      const lb4 a = *(const lb4*)(p + at(fr, 8 * kd + g)), b = *(const lb4*)(p + at(fr, 8 * kd + 4 + g));
-      f[k] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
+    for (int k = 0; k < IN; ++k) f[k] = *(const lb8*)(tile + k * PART + rt * 16 * PITCH + at(fr, 8 * kd + 2 * g));
   }
-  // the transpose: column 16 ct + lane % 16, rows {4 g ..+3} and {16 + 4 g ..+3}
-  static __device__ __forceinline__ void col(const char* tile, int ct, int lane, lb8 (&f)[IN]) {
+  // transposed: rows {4 g ..+3} and {16 + 4 g ..+3} of the column that is lane % 16 of the four half pieces u, u + step ...
+  static __device__ __forceinline__ void col(const char* tile, int u0, int step, int lane, lb8 (&f)[IN]) {
 #pragma unroll
     for (int k = 0; k < IN; ++k) {
-      const char* const p = tile + k * PART + at(4 * (lane >> 4) + ((lane & 15) >> 2), 4 * ct + (lane & 3));
+      const char* const p = tile + k * PART + at(4 * (lane >> 4) + ((lane & 15) >> 2), u0 + step * (lane & 3));
       union { struct { s16x4 a, b; } s; lb8 v; } u;
       u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)p);
       u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_s16x4*)(p + 16 * PITCH));
       f[k] = u.v;
     }
   }
+  static __device__ __forceinline__ void col_values(const char* tile, int n0, int lane, lb8 (&f)[IN]) { col(tile, n0 / 4, 1, lane, f); }         // column n0 + lane % 16
+  static __device__ __forceinline__ void col_state(const char* tile, int t, int lane, lb8 (&f)[IN]) { col(tile, 8 * (t >> 1) + (t & 1), 2, lane, f); }       // the state's tile t
 };
+__device__ __forceinline__ int lin_channel(int t, int g, int i) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i; }         // of row 4 g + i of tile t
 template <int IN> __device__ __forceinline__ float lin_value(const lb8 (&f)[IN], int i) {       // the element that the parts stand for
   float x = (float)f[0][i];
 #pragma unroll
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = Tile::IN == 1 ? 2 * HD : 4 * HD + 16;            // OP: pitch of the result's tile, bytes
   constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
-  constexpr int WAVES = HD / 16, PP = 72, PPART = C * PP;        // scores: 32 rows of 32 bf16 at a pitch of 18 words (16 rows, 16 lanes: all banks)
+  constexpr int WAVES = HD / 16, PP = 80, PPART = C * PP;        // scores: rows of 32 bf16 at a pitch of 20 words (16 rows, 16 lanes: all banks)
   __shared__ __attribute__((aligned(16))) char sm[(STATE ? 2 : 3) * Tile::BYTES + (STATE ? 0 : C * OP + L::MID * PPART)];
   char* const sK = sm;
   char* const sV = sm + Tile::BYTES;
@@ -292,11 +294,16 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
     }
   };
 
+  if constexpr (!STATE) {                                        // the first queries' weights of the second tile of keys are zeros for good
+#pragma unroll
+    for (int k = 0; k < L::MID; ++k)
+      if (tid < 64) *(lin_half*)(sP + k * PPART + fr * PP + 16 * g + 8) = (lin_half){0u, 0u};
+  }
   offsets_in(C);
   if constexpr (!STATE) offsets(ao, os, C);
   if (from < upto) fetch(upto - from < C ? upto - from : C);
 
-  f32x4 S[ND];                                                   // S[t][i]: row 16 t + 4 g + i of the state, column n0 + fr
+  f32x4 S[ND];                                                   // S[t][i]: row lin_channel(t, g, i) of the state, column n0 + fr
 #pragma unroll
   for (int t = 0; t < ND; ++t) S[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if constexpr (!STATE) {
@@ -307,7 +314,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       for (int t = 0; t < ND; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int d = 16 * t + 4 * g + i;
+          const int d = lin_channel(t, g, i);
           S[t][i] = f0 * (r.first_t ? p[(n0 + fr) * HD + d] : p[d * HD + n0 + fr]);
         }
     }
@@ -324,9 +331,11 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
           if (!r.ws_t) x[u][t] = *(const f32x4*)(w + (((tid >> 6) * ND + t) * 64 + lane) * 4);
-          else                                                   // element (16 t + 4 g + i, n0 + fr) of the transpose
+          else {                                                 // element (row, column) = (c, d) of the role that left it
+            const int c = n0 + fr, d = lin_channel(t, g, 0), tile = 2 * (c >> 5) + (c >> 2 & 1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][t][i] = w[((t * ND + (tid >> 6)) * 64 + (fr >> 2) * 16 + 4 * g + i) * 4 + (fr & 3)];
+            for (int i = 0; i < 4; ++i) x[u][t][i] = w[(((d >> 4) * ND + tile) * 64 + (c >> 3 & 3) * 16 + (d & 15) + i) * 4 + (c & 3)];
+          }
         }
       }
 #pragma unroll
@@ -386,7 +395,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
           unsigned w[L::MID][2];
           lin_split<L::MID, 2>(x, w);
 #pragma unroll
-          for (int k = 0; k < L::MID; ++k) *(lin_half*)(sP + k * PPART + (16 * ti + fr) * PP + 32 * e + 8 * g) = (lin_half){w[k][0], w[k][1]};
+          for (int k = 0; k < L::MID; ++k) *(lin_half*)(sP + k * PPART + (16 * ti + fr) * PP + 16 * g + 8 * e) = (lin_half){w[k][0], w[k][1]};
         }
 #pragma unroll
       for (int kd = 0; kd < NK; ++kd) {
@@ -403,7 +412,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       acc[1] *= lrow * l16;
     }
     lb8 vf[L::IN];
-    Tile::col(sV, n0 / 16, lane, vf);
+    Tile::col_values(sV, n0, lane, vf);
     if (!END || !ends || r.last) {
       const int e = END && ends ? c - off : C;                   // the state behind the last row itself, or as the next row sees it
       const float le = END ? lin_pow(l2, e) : lC;
@@ -413,7 +422,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       if (!END || e == C) {                                      // l^(C - j), j = 16 tile + 4 g + i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = lin_value(vf, i) * l16 * wv[i];
+          x[i] = lin_value(vf, i) * (l16 * wv[i]);
           x[4 + i] = lin_value(vf, 4 + i) * wv[i];
         }
       } else {
@@ -428,7 +437,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
         lb8 kf[L::IN];
-        Tile::col(sK, t, lane, kf);
+        Tile::col_state(sK, t, lane, kf);
         S[t] = lin_mma(kf, p, S[t]);
       }
     }
@@ -438,11 +447,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       for (int ti = 0; ti < 2; ++ti) {
         lb8 p[L::MID];
 #pragma unroll
-        for (int k = 0; k < L::MID; ++k) {
-          const char* const at = sP + k * PPART + (16 * ti + fr) * PP + 8 * g;
-          const lb4 lo = *(const lb4*)at, hi = ti ? *(const lb4*)(at + 32) : (lb4){};
-          p[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
+        for (int k = 0; k < L::MID; ++k) p[k] = *(const lb8*)(sP + k * PPART + (16 * ti + fr) * PP + 16 * g);
         acc[ti] = lin_mma(vf, p, acc[ti]);
       }
     }
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[(16 * t + 4 * g + i) * HD + n0 + fr] = S[t][i];
+      for (int i = 0; i < 4; ++i) p[lin_channel(t, g, i) * HD + n0 + fr] = S[t][i];
   }
 }
 
