@@ -146,6 +146,12 @@ template <typename T, int HD> struct LinTile {
   static __device__ __forceinline__ void col_state(const char* tile, int t, int lane, lb8 (&f)[IN]) { col(tile, 8 * (t >> 1) + (t & 1), 2, lane, f); }       // the state's tile t
 };
 __device__ __forceinline__ int lin_channel(int t, int g, int i) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i; }         // of row 4 g + i of tile t
+// 16 bytes of each lane from base + off to lds + 16 lane, without a register in between.  In asm, so that the compiler does not wait for them in
+// front of every read from LDS: what waits is lin_wait, with the number of memory operations that are surely younger.
+__device__ __forceinline__ void lin_dma(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void lin_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 template <int IN> __device__ __forceinline__ float lin_value(const lb8 (&f)[IN], int i) {       // the element that the parts stand for
   float x = (float)f[0][i];
 #pragma unroll
@@ -198,11 +204,12 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
   constexpr int WAVES = HD / 16, PP = 80, PPART = C * PP;        // scores: rows of 32 bf16 at a pitch of 20 words (16 rows, 16 lanes: all banks)
-  __shared__ __attribute__((aligned(16))) char sm[(STATE ? 2 : 3) * Tile::BYTES + (STATE ? 0 : C * OP + L::MID * PPART)];
-  char* const sK = sm;
-  char* const sV = sm + Tile::BYTES;
-  char* const sQ = sm + (STATE ? 0 : 2) * Tile::BYTES;
-  char* const sO = sm + (STATE ? 0 : 3) * Tile::BYTES;
+  // 16-bit operands go straight to LDS, into two stages of tiles in turn; 32-bit ones are split on the way, through registers.  (Two chunks
+  // ahead instead of one: 0 to 3 % slower.)
+  constexpr bool DMA = L::IN == 1;
+  constexpr int LOADS = STATE ? 2 : 3, STAGE = LOADS * Tile::BYTES;
+  __shared__ __attribute__((aligned(16))) char sm[(DMA ? 2 : 1) * STAGE + (STATE ? 0 : C * OP + L::MID * PPART)];
+  char* const sO = sm + (STATE ? 0 : (DMA ? 2 : 1) * STAGE);
   char* const sP = sO + (STATE ? 0 : C * OP);
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
@@ -259,28 +266,36 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   const bool o32 = r.o32;
   lin_raw pq[NU], pk[NU], pv[NU];                                // the next chunk's tiles, in flight during this one's math
   unsigned aq[NU], ak[NU], av[NU], ao[NU];
-  auto offsets = [&](unsigned (&off)[NU], long long stride, int c) __attribute__((always_inline)) {
+  auto offsets = [&](unsigned (&off)[NU], long long stride, int c, bool in) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int at = tid + u * THREADS, i = at / CPR < c ? at / CPR : c - 1;
-      off[u] = (unsigned)(rev ? c - 1 - i : i) * (unsigned)stride + (at % CPR) * 16;
+      off[u] = (unsigned)(rev ? c - 1 - i : i) * (unsigned)stride + ((at % CPR) ^ (in && DMA ? Tile::swz(at / CPR) : 0)) * 16;
     }
   };
   auto offsets_in = [&](int c) __attribute__((always_inline)) {
-    if constexpr (!STATE) offsets(aq, qs, c);
-    offsets(ak, ks, c);
-    offsets(av, vs, c);
+    if constexpr (!STATE) offsets(aq, qs, c, true);
+    offsets(ak, ks, c, true);
+    offsets(av, vs, c, true);
   };
-  auto fetch = [&](int c) __attribute__((always_inline)) {
+  const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)sm + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+  auto fetch = [&](int c, int stage) __attribute__((always_inline)) {
     if (c < C) {
       offsets_in(c);
       if (rev) { bq += (C - c) * qs; bk += (C - c) * ks; bv += (C - c) * vs; }
     }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      if constexpr (!STATE) pq[u] = *(const lin_raw*)(bq + aq[u]);
-      pk[u] = *(const lin_raw*)(bk + ak[u]);
-      pv[u] = *(const lin_raw*)(bv + av[u]);
+      if constexpr (DMA) {
+        const unsigned to = lds + stage + u * THREADS * 16;
+        lin_dma(bk, ak[u], to);
+        lin_dma(bv, av[u], to + Tile::BYTES);
+        if constexpr (!STATE) lin_dma(bq, aq[u], to + 2 * Tile::BYTES);
+      } else {
+        if constexpr (!STATE) pq[u] = *(const lin_raw*)(bq + aq[u]);
+        pk[u] = *(const lin_raw*)(bk + ak[u]);
+        pv[u] = *(const lin_raw*)(bv + av[u]);
+      }
     }
     bq += dq; bk += dk; bv += dv;
   };
@@ -288,9 +303,9 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int at = tid + u * THREADS, i = at / CPR, e = at % CPR;
-      if constexpr (!STATE) Tile::put(sQ, i, e, pq[u]);
-      Tile::put(sK, i, e, pk[u]);
-      Tile::put(sV, i, e, pv[u]);
+      Tile::put(sm, i, e, pk[u]);
+      Tile::put(sm + Tile::BYTES, i, e, pv[u]);
+      if constexpr (!STATE) Tile::put(sm + 2 * Tile::BYTES, i, e, pq[u]);
     }
   };
 
@@ -300,8 +315,9 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       if (tid < 64) *(lin_half*)(sP + k * PPART + fr * PP + 16 * g + 8) = (lin_half){0u, 0u};
   }
   offsets_in(C);
-  if constexpr (!STATE) offsets(ao, os, C);
-  if (from < upto) fetch(upto - from < C ? upto - from : C);
+  if constexpr (!STATE) offsets(ao, os, C, false);
+  auto rows_at = [&](int t) __attribute__((always_inline)) { return upto - t < C ? upto - t : C; };
+  if (from < upto) fetch(rows_at(from), 0);
 
   f32x4 S[ND];                                                   // S[t][i]: row lin_channel(t, g, i) of the state, column n0 + fr
 #pragma unroll
@@ -361,11 +377,20 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   const float l16 = lin_uniform(lin_pow(l2, 16)), lC = lin_uniform(lin_pow(l2, C)), lrow = r.s_inter * lin_pow(l2, fr);
 
   // one chunk of c rows; END: the segment's last one, which may be short and may end the sequence
-  auto chunk = [&](auto end, int t0, int c) __attribute__((always_inline)) {
+  auto chunk = [&](auto end, int t0, int c, int stage) __attribute__((always_inline)) {
     constexpr bool END = decltype(end)::value;
-    place();
+    const char* const sK = sm + stage;
+    const char* const sV = sK + Tile::BYTES;
+    const char* const sQ = sK + (STATE ? 0 : 2) * Tile::BYTES;
+    if constexpr (DMA) {
+      // Younger than this chunk's loads are the rows that the last chunk has stored.  Where every operand is read by one workgroup, memory is
+      // what bounds the kernel, and it is faster if a workgroup's stores are through before it goes on (64 x 2000 rows: 229 us against 240);
+      // where roles or shared heads meet in the L2 it is not (training pair of 140 rows 161 against 156, ragged shared heads 108 against 103).
+      if (END || STATE || o32 || t0 == from || a.roles * a.rep == 1) lin_wait<0>();
+      else lin_wait<NU>();
+    } else place();
     __syncthreads();
-    if constexpr (!END) fetch(upto - t0 - C < C ? upto - t0 - C : C);
+    if constexpr (!END) fetch(rows_at(t0 + C), DMA ? STAGE - stage : 0);
     f32x4 acc[2];                                                // results of the two query tiles
     acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if constexpr (!STATE) {
@@ -441,8 +466,8 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
         S[t] = lin_mma(kf, p, S[t]);
       }
     }
+    if constexpr (!STATE || !DMA) __syncthreads();
     if constexpr (!STATE) {
-      __syncthreads();
 #pragma unroll
       for (int ti = 0; ti < 2; ++ti) {
         lb8 p[L::MID];
@@ -461,13 +486,13 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
         }
       }
     }
-    __syncthreads();
     if constexpr (!STATE) {
+      __syncthreads();
       // whole rows, 16 bytes a lane: 8-byte pieces straight from the accumulators cost 10 % of the launch.  Past the L2, which the
       // operands need: 2 to 5 % on every long case.
       if (!o32) {
         if (END && c < C) {
-          offsets(ao, os, c);
+          offsets(ao, os, c, false);
           if (rev) bo += (C - c) * os;
         }
 #pragma unroll
@@ -479,9 +504,12 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       }
     }
   };
-  int t0 = from;
-  for (; t0 + C < upto; t0 += C) chunk(std::false_type{}, t0, C);
-  if (t0 < upto) chunk(std::true_type{}, t0, upto - t0);
+  int t0 = from, stage = 0;
+  for (; t0 + C < upto; t0 += C) {
+    chunk(std::false_type{}, t0, C, stage);
+    if constexpr (DMA) stage = STAGE - stage;
+  }
+  if (t0 < upto) chunk(std::true_type{}, t0, upto - t0, stage);
   if constexpr (STATE) {
     f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
 #pragma unroll
