@@ -13,8 +13,8 @@
 //
 // One workgroup owns a (sequence, head) or a segment of one and walks its chunks with the state in registers.  A wave owns 16 columns
 // of v: the whole HD x 16 slice of the state lives in its MFMA accumulators, whose layout IS the A operand of Y^T q, so the state never
-// passes through LDS.  The scores do: a wave forms one 16 x 16 tile of them for all waves (each wave forming all of them instead: 183 us
-// against 173 for the training pair of 152-row clips, 323 against 285 with 128 channels).
+// passes through LDS.  The scores do: a wave forms one 16 x 16 tile of them for all waves (each wave forming all of them instead: 6 % more
+// for the training pair of 140-row clips, 13 % with 128 channels).
 // Products are issued swapped (P^T = K Q^T, O^T = V^T P^T + Y^T Q^T): see a2v_attn.hip for the layout argument.
 //
 // All products run on the bf16 matrix cores, fp32 values as sums of bf16 parts of 8 bits each (x = hi + mid + lo exactly; the products of
@@ -61,12 +61,12 @@ struct LinArgs {
 };
 #define LIN_GRID_Y 32768
 // Sequences of up to so many segments: a segment sums the states in front of it itself.  More: the scan kernel does (one recording of 64
-// segments: 16 heads x 64 x 16 KB for each of them).  One clip of 16 segments: 23.0 us with the scan kernel, 17.8 without.
+// segments: 16 heads x 64 x 16 KB for each of them).  One clip of 16 segments: 21.2 us with the scan kernel, 16.1 without.
 #define LIN_INLINE 16
 
-#define LIN_C 32              /* rows of a chunk: two tiles of 16.  64 rows pay the state's share half as often and meet half the barriers, but
-                                 take 168 registers in place of 128: 3 workgroups on a CU, not 4 (512 x 2000 rows: 248 us against 223; the
-                                 training pair 208 against 168) */
+// Rows of a chunk: two tiles of 16.  64 rows pay the state's share half as often and meet half the barriers, but take 168 registers in place
+// of 128: 3 workgroups on a CU, not 4 (64 clips of 2000 rows 11 % slower, the training pair of 140-row clips 24 %).
+#define LIN_C 32
 template <typename T> struct LinT;
 template <> struct LinT<__bf16> { static constexpr int IN = 1, MID = 2, V = 8; };      // parts of the operands, of scores and states; elements of 16 bytes
 template <> struct LinT<float> { static constexpr int IN = 3, MID = 3, V = 4; };
@@ -194,6 +194,14 @@ __device__ __forceinline__ float lin_log2(const float* slopes, int h) {
 __device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
+// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 229 us, 4.6 TB/s, where a large copy reaches 5.1 -- memory.
+// The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU; the vector pipe issues half of that time (splitting the state and the
+// weighted values into parts is half of its 140 instructions a chunk and wave) and the matrix pipe a quarter, and four waves to a SIMD that
+// meet at three barriers do not fill the rest.  A recording reads k and v twice (state kernel: 5.5 TB/s), and a long backward's dq, which
+// runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory instead of 4.
+// Registers: 128 with 16-bit operands, four waves to a SIMD; three parts take 166, three waves (two: 90 us against 84 for the training pair
+// of 2 x 2000 rows in fp32), with 128 channels two.
+//
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 // EXACT: the state is a result (or might be: out does not depend on that) and keeps all of its 32 bits with a third part of the values.
 template <typename T, int HD, bool STATE, bool EXACT>
@@ -575,7 +583,8 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* dk32, const 
 }
 
 // One token of each of N streams, the state updated in place: state once in, once out, everything else is negligible (HBM, or latency
-// where N H is small).  A thread holds four neighbouring columns of HD * HD / 1024 rows of the state.
+// where N H is small: 256 streams of 16 heads of 64 channels 22.5 us, 6.1 TB/s of state, part of it out of the Infinity Cache; one stream
+// 3.2 us).  A thread holds four neighbouring columns of HD * HD / 1024 rows of the state.
 // slots[n] names the state of row n.  Rows that name the same slot are successive tokens of one stream, in row order: the workgroup of
 // the first of them takes them all (the others find an earlier row and leave), so there is no race and no order left open.  A slot
 // outside [0, n_slots) leaves every state alone and gives a row of zeros (padding rows of a captured graph).
@@ -642,8 +651,8 @@ __global__ __launch_bounds__(256) void lin_step_kernel(LinStep a) {
 
 // Rows of a segment.  Enough (sequence, head) pairs: one segment each, k and v read once.  Fewer: the axis is cut until LIN_WGS
 // workgroups run, which costs a second pass over k and v; not below 4 HD rows, where writing and reading the states (HD * HD * 4 bytes)
-// costs as much as it gives (4 clips of 2000 rows, 16 heads: 34.4 us at 256 rows, 36.4 at 128), except that fewer than a workgroup for
-// each compute unit are worse still: then 2 HD (one such clip: 26.8 us at 256 rows, 23.6 at 128, 24.9 at 64).
+// costs as much as it gives (4 clips of 2000 rows, 16 heads: 26 us at 256 rows, 33 at 128), except that fewer than a workgroup for
+// each compute unit are worse still: then 2 HD (one such clip: 19.0 us at 256 rows, 16.1 at 128, 23.4 at 64).
 static int lin_seg(int B, long long rows, int S, int H, int HD, bool packed, int C) {
   const long long all = packed ? rows : S;
   if (!packed && (long long)B * H >= LIN_WGS / 2) return all > 0 ? cdiv(all, C) * C : C;
