@@ -533,8 +533,8 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 
 // ws[slot] := the state in front of segment p from the segments before it: carried through the sequence's slots in order, one thread to an
 // element (any order of them: the waves' register image), eight loads in flight.  The part of `first` is added by the kernel that starts
-// from it.  At most LIN_SCANS sequences are in work at a time: short ones of a packed batch, which have nothing to scan, cost a look each
-// (37 of them with a workgroup apiece: 4.7 us).
+// from it.  LIN_SCANS groups of workgroups take the sequences in turn, so that the launch does not grow with their number.  (A packed batch of
+// short sequences, which have nothing to scan, pays the launch, 4.6 us: their lengths are on the device.)
 #define LIN_SCANS 8
 __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
   const int per = a.H * HH / 256, b0 = blockIdx.x / per;
