@@ -195,8 +195,8 @@ __device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
 // What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 229 us, 4.6 TB/s, where a large copy reaches 5.1 -- memory.
-// The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU; the vector pipe issues half of that time (splitting the state and the
-// weighted values into parts is half of its 140 instructions a chunk and wave) and the matrix pipe a quarter, and four waves to a SIMD that
+// The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU; the vector pipe issues 71 % of that time (splitting the state and the
+// weighted values into parts is half of its 140 instructions a chunk and wave), the matrix pipe 28 %, and four waves to a SIMD that
 // meet at three barriers do not fill the rest.  A recording reads k and v twice (state kernel: 5.5 TB/s), and a long backward's dq, which
 // runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory instead of 4.
 // Registers: 128 with 16-bit operands, four waves to a SIMD; three parts take 166, three waves (two: 90 us against 84 for the training pair

@@ -10,6 +10,9 @@ before the one rounding:
   norm and rotation       sum of HD squares (HD 2^-24, halved by the root), root and products (8 x 2^-24), sine and cosine (2^-22):
                           c = 2^-18 for HD <= 128
 """
+import contextlib
+import threading
+
 import pytest
 import torch
 
@@ -497,7 +500,7 @@ def test_linear_attention_non_finite_rows_do_not_reach_the_past(ops):
 
 
 @gpu
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("N,H,HK,HD,pool", [(1, 1, 1, 64, 0), (5, 4, 2, 32, 0), (7, 3, 3, 128, 11), (300, 2, 1, 64, 301)])
 def test_linear_attention_step(ops, N, H, HK, HD, pool, dtype):
     qkv = rnd(N, H + 2 * HK, HD, seed=1, dtype=dtype)
@@ -506,7 +509,8 @@ def test_linear_attention_step(ops, N, H, HK, HD, pool, dtype):
     state = rnd(P, H, HD, HD, seed=2)
     slots = torch.randperm(P, generator=torch.Generator().manual_seed(3))[:N].to(torch.int32) if pool else None
     sd, x = state.cuda(), qkv.cuda()
-    out = ops.linear_attention_step(x[:, :H], x[:, H:H + HK], x[:, H + HK:], alibi(H).cuda(), sd, slots=slots.cuda() if pool else None, scale=0.9)
+    with ops.half_library() if dtype == torch.float16 else contextlib.nullcontext():
+        out = ops.linear_attention_step(x[:, :H], x[:, H:H + HK], x[:, H + HK:], alibi(H).cuda(), sd, slots=slots.cuda() if pool else None, scale=0.9)
     for n in range(min(N, 40)):
         s = int(slots[n]) if pool else n
         want = ref_linear(q[n:n + 1].double(), k[n:n + 1].double(), v[n:n + 1].double(), alibi(H), 0.9, state[s].double())
@@ -659,6 +663,72 @@ def test_streams_and_captured_graphs(ops):
             torch.cuda.synchronize()
             for a, b, c in zip(want, res, eager):
                 assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_replays_follow_the_offsets_on_the_device(ops, dtype):
+    """a captured packed forward and backward of shared heads, replayed with other inputs and other sequences in the same buffers: each
+    replay equals an eager call, rows outside every sequence are zeros again"""
+    T, H, HK, HD = 1300, 4, 2, 64
+    lay = [(0, 700, 700, 1300), (40, 41, 900, 1200), (0, 0, 1300, 1300), (1299, 1299, 1299, 1299)]
+    q, k, v, do = (rnd(1, T, h, HD, seed=i, dtype=dtype).cuda() for i, h in enumerate((H, HK, HK, H)))
+    cu, sl = torch.tensor(lay[0], dtype=torch.int32, device="cuda"), alibi(H, 0.01).cuda()
+    st, ds = (rnd(3, H, HD, HD, seed=i).cuda() for i in (7, 8))
+
+    def once():
+        out, last = ops.linear_attention_fwd(q, k, v, sl, state=st, cu_seqlens=cu, want_state=True)
+        return (out, last, *ops.linear_attention_bwd(q, k, v, sl, do, state=st, d_state=ds, cu_seqlens=cu))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once()
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = once()
+    for i, c in enumerate(lay + lay[:1]):
+        cu.copy_(torch.tensor(c, dtype=torch.int32))
+        q.copy_(rnd(1, T, H, HD, seed=20 + i, dtype=dtype))
+        for t in res:
+            t.fill_(9.0)
+        g.replay()
+        want = once()
+        torch.cuda.synchronize()
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+        for t in (res[0], res[2], res[3], res[4]):
+            assert not t[0, :c[0]].any() and not t[0, c[-1]:].any()
+
+
+@gpu
+def test_calls_on_two_streams_and_from_two_threads(ops):
+    """calls in flight at the same time have their own workspaces"""
+    H, HD = 4, 64
+    sl = alibi(H).cuda()
+    sets = [[t.cuda() for t in lin_case(1, S, H, H, HD, torch.bfloat16, seed=S)] for S in (3000, 2500)]
+
+    def call(x, n=1):
+        for _ in range(n):
+            r = ops.linear_attention_fwd(x[0], x[1], x[2], sl, state=x[4], want_state=True) + \
+                ops.linear_attention_bwd(x[0], x[1], x[2], sl, x[3], state=x[4], d_state=x[5])
+        return r
+    want = [call(x) for x in sets]
+    torch.cuda.synchronize()
+    streams, got, errors = [torch.cuda.Stream() for _ in sets], [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                got[i] = call(sets[i], 20)
+        except Exception as e:      # noqa: BLE001 (shown below)
+            errors.append(e)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 @gpu
