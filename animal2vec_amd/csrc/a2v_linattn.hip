@@ -84,11 +84,31 @@ template <int PARTS, int N> __device__ __forceinline__ void lin_split(const floa
     }
   }
 }
-template <int PARTS> __device__ __forceinline__ void lin_split8(const float* x, lb8 (&f)[PARTS]) {
-  union { unsigned w[PARTS][4]; lb8 v[PARTS]; } u;
-  lin_split<PARTS, 4>(x, u.w);
+// The same for a pair of tiles of 16 x 16 in the accumulators' layout (row 4 g + i, column fr), which gives the operand of 32 rows and 16 columns:
+// its inner index is row 4 g + i of tile h at element 4 h + i of lane group g.  What a part leaves is x - part, a product with minus one's
+// matrix: exact, and one matrix instruction in place of eight vector ones, which are what these kernels run out of.  (A part that is not
+// finite spoils its column of the tiles, whose sums it would enter as well.)
+struct LinMinus { lb8 of[2]; };                                  // row fr of tile h: -1 at its own element
+__device__ __forceinline__ LinMinus lin_minus(int fr, int g) {
+  LinMinus m;
 #pragma unroll
-  for (int k = 0; k < PARTS; ++k) f[k] = u.v[k];
+  for (int i = 0; i < 4; ++i) {
+    const __bf16 v = fr == 4 * g + i ? (__bf16)-1.f : (__bf16)0.f;
+    m.of[0][i] = m.of[1][4 + i] = v;
+    m.of[0][4 + i] = m.of[1][i] = (__bf16)0.f;
+  }
+  return m;
+}
+template <int PARTS> __device__ __forceinline__ void lin_split_tiles(f32x4 a, f32x4 b, const LinMinus& minus, lb8 (&f)[PARTS]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    const lb4 lo = __builtin_convertvector(a, lb4), hi = __builtin_convertvector(b, lb4);
+    f[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    if (k + 1 < PARTS) {
+      a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus.of[0], f[k], a, 0, 0, 0);
+      b = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus.of[1], f[k], b, 0, 0, 0);
+    }
+  }
 }
 // c += a b over 32 of the inner index, a and b in parts; products below the last part of the longer one are left out
 template <int NA, int NB> __device__ __forceinline__ f32x4 lin_mma(const lb8 (&a)[NA], const lb8 (&b)[NB], f32x4 c) {
@@ -372,6 +392,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
     }
   }
 
+  const LinMinus minus = lin_minus(fr, g);
   // l^(i - j) scale for a query column fr and key rows 4 g + i: inside a tile, and one tile apart
   const float scale = r.s_inter * r.s_state;
   float w0[4], w1[4], wv[4];
@@ -432,11 +453,8 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
         }
 #pragma unroll
       for (int kd = 0; kd < NK; ++kd) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { x[i] = S[2 * kd][i]; x[4 + i] = S[2 * kd + 1][i]; }
         lb8 y[L::MID];
-        lin_split8<L::MID>(x, y);
+        lin_split_tiles<L::MID>(S[2 * kd], S[2 * kd + 1], minus, y);
         if constexpr (!HOLD) { query(0, kd); query(1, kd); }
         acc[0] = lin_mma(y, qf[0][kd], acc[0]);
         acc[1] = lin_mma(y, qf[1][kd], acc[1]);
@@ -451,22 +469,22 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       const float le = END ? lin_pow(l2, e) : lC;
 #pragma unroll
       for (int t = 0; t < ND; ++t) S[t] *= le;
-      float x[8];
+      f32x4 x[2];
       if (!END || e == C) {                                      // l^(C - j), j = 16 tile + 4 g + i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = lin_value(vf, i) * (l16 * wv[i]);
-          x[4 + i] = lin_value(vf, 4 + i) * wv[i];
+          x[0][i] = lin_value(vf, i) * (l16 * wv[i]);
+          x[1][i] = lin_value(vf, 4 + i) * wv[i];
         }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int j = 4 * g + 16 * (i >> 2) + (i & 3);
-          x[i] = j < c ? lin_value(vf, i) * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
+          x[i >> 2][i & 3] = j < c ? lin_value(vf, i) * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
         }
       }
       lb8 p[EXACT ? 3 : L::MID];
-      lin_split8<EXACT ? 3 : L::MID>(x, p);
+      lin_split_tiles<EXACT ? 3 : L::MID>(x[0], x[1], minus, p);
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
         lb8 kf[L::IN];
