@@ -214,10 +214,9 @@ __device__ __forceinline__ float lin_log2(const float* slopes, int h) {
 __device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
-// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 229 us, 4.6 TB/s, where a large copy reaches 5.1 -- memory.
-// The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU; the vector pipe issues 71 % of that time (splitting the state and the
-// weighted values into parts is half of its 140 instructions a chunk and wave), the matrix pipe 28 %, and four waves to a SIMD that
-// meet at three barriers do not fill the rest.  A recording reads k and v twice (state kernel: 5.5 TB/s), and a long backward's dq, which
+// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 227 us, 4.6 TB/s, where a large copy reaches 5.1 -- memory.
+// The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU, the vector pipe busy for 59 % of it and the matrix pipe for 35 %; a chunk is
+// a chain of LDS reads, matrix and vector steps of 2 us, and four waves to a SIMD do not hide all of it.  A recording reads k and v twice (state kernel: 5.2 TB/s), and a long backward's dq, which
 // runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory instead of 4.
 // Registers: 128 with 16-bit operands, four waves to a SIMD; three parts take 166, three waves (two: 90 us against 84 for the training pair
 // of 2 x 2000 rows in fp32), with 128 channels two.
