@@ -11,7 +11,8 @@
 //     dk_t = D_t v_t           backwards,        (q, k, v) := (v, scale do, q),  state D^T
 // so ONE kernel does all four: a "role" names its operands, its direction and where the scale goes.
 //
-// One workgroup owns a (sequence, head) or a segment of one and walks its chunks with the state in registers.  A wave owns 16 columns
+// One workgroup owns a (sequence, head) or a segment of one -- or the same of two or four neighbouring heads, for longer pieces of rows -- and
+// walks its chunks with the state in registers.  A wave owns 16 columns
 // of v: the whole HD x 16 slice of the state lives in its MFMA accumulators, whose layout IS the A operand of Y^T q, so the state never
 // passes through LDS.  The scores do: a wave forms one 16 x 16 tile of them for all waves (each wave forming all of them instead: 6 % more
 // for the training pair of 140-row clips, 13 % with 128 channels).
@@ -146,10 +147,10 @@ template <typename T, int HD> struct LinTile {
       for (int k = 0; k < IN; ++k) *(lin_half*)(tile + k * PART + at(r, c)) = (lin_half){w[k][0], w[k][1]};
     }
   }
-  // 8 elements of row 16 rt + fr at columns 32 kd + 8 g ..+7
-  static __device__ __forceinline__ void row(const char* tile, int rt, int fr, int kd, int g, lb8 (&f)[IN]) {
+  // 8 elements of row 16 rt + fr, from half piece u0 on
+  static __device__ __forceinline__ void row(const char* tile, int rt, int fr, int u0, lb8 (&f)[IN]) {
 #pragma unroll
-    for (int k = 0; k < IN; ++k) f[k] = *(const lb8*)(tile + k * PART + rt * 16 * PITCH + at(fr, 8 * kd + 2 * g));
+    for (int k = 0; k < IN; ++k) f[k] = *(const lb8*)(tile + k * PART + rt * 16 * PITCH + at(fr, u0));
   }
   // transposed: rows {4 g ..+3} and {16 + 4 g ..+3} of the column that is lane % 16 of the four half pieces u, u + step ...
   static __device__ __forceinline__ void col(const char* tile, int u0, int step, int lane, lb8 (&f)[IN]) {
@@ -162,8 +163,6 @@ template <typename T, int HD> struct LinTile {
       f[k] = u.v;
     }
   }
-  static __device__ __forceinline__ void col_values(const char* tile, int n0, int lane, lb8 (&f)[IN]) { col(tile, n0 / 4, 1, lane, f); }         // column n0 + lane % 16
-  static __device__ __forceinline__ void col_state(const char* tile, int t, int lane, lb8 (&f)[IN]) { col(tile, 8 * (t >> 1) + (t & 1), 2, lane, f); }       // the state's tile t
 };
 __device__ __forceinline__ int lin_channel(int t, int g, int i) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i; }         // of row 4 g + i of tile t
 // 16 bytes of each lane from base + off to lds + 16 lane, without a register in between.  In asm, so that the compiler does not wait for them in
@@ -214,45 +213,49 @@ __device__ __forceinline__ float lin_log2(const float* slopes, int h) {
 __device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
-// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 227 us, 4.6 TB/s, where a large copy reaches 5.1 -- memory.
+// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 212 us, 4.95 TB/s, where a large copy reaches 5.2 -- memory.
 // The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU, the vector pipe busy for 59 % of it and the matrix pipe for 35 %; a chunk is
-// a chain of LDS reads, matrix and vector steps of 2 us, and four waves to a SIMD do not hide all of it.  A recording reads k and v twice (state kernel: 5.2 TB/s), and a long backward's dq, which
-// runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory instead of 4.
+// a chain of LDS reads, matrix and vector steps of 2 us, and four waves to a SIMD do not hide all of it.  A recording reads k and v twice, and
+// a long backward's dq, which runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory
+// instead of 4.
 // Registers: 128 with 16-bit operands, four waves to a SIMD; three parts take 166, three waves (two: 90 us against 84 for the training pair
 // of 2 x 2000 rows in fp32), with 128 channels two.
 //
+// HEADS: neighbouring heads of a workgroup (lin_wide), each with waves, scores and state of its own, side by side in the tiles' rows.
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
 // EXACT: the state is a result (or might be: out does not depend on that) and keeps all of its 32 bits with a third part of the values.
-template <typename T, int HD, bool STATE, bool EXACT>
-__global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) void lin_kernel(LinArgs a) {
+template <typename T, int HD, int HEADS, bool STATE, bool EXACT>
+__global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
-  typedef LinTile<T, HD> Tile;
-  constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = HD * 4, OP = Tile::IN == 1 ? 2 * HD : 4 * HD + 16;            // OP: pitch of the result's tile, bytes
-  constexpr int CPR = HD / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
+  constexpr int W = HD * HEADS;                                  // channels of a row of the tiles
+  typedef LinTile<T, W> Tile;
+  constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = W * 4, OP = Tile::IN == 1 ? 2 * W : 4 * W + 16;            // OP: pitch of the result's tile, bytes
+  constexpr int CPH = HD / L::V, CPR = W / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
   constexpr int WAVES = HD / 16, PP = 80, PPART = C * PP;        // scores: rows of 32 bf16 at a pitch of 20 words (16 rows, 16 lanes: all banks)
   // 16-bit operands go straight to LDS, into two stages of tiles in turn; 32-bit ones are split on the way, through registers.  (Two chunks
   // ahead instead of one: 0 to 3 % slower.)
   constexpr bool DMA = L::IN == 1;
   constexpr int LOADS = STATE ? 2 : 3, STAGE = LOADS * Tile::BYTES;
-  __shared__ __attribute__((aligned(16))) char sm[(DMA ? 2 : 1) * STAGE + (STATE ? 0 : C * OP + L::MID * PPART)];
+  __shared__ __attribute__((aligned(16))) char sm[(DMA ? 2 : 1) * STAGE + (STATE ? 0 : C * OP + HEADS * L::MID * PPART)];
   char* const sO = sm + (STATE ? 0 : (DMA ? 2 : 1) * STAGE);
-  char* const sP = sO + (STATE ? 0 : C * OP);
+  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int me = HEADS == 1 ? 0 : wave / WAVES, wi = wave - me * WAVES, n0 = wi * 16, u0 = me * (HD / 4);       // head of the workgroup, wave of the head
+  char* const sP = sO + (STATE ? 0 : C * OP + me * L::MID * PPART);
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
   const int nr = STATE ? a.roles_state : a.roles, in = blockIdx.x >> 3, turn = blockIdx.z * LIN_GRID_Y + blockIdx.y;
   // Neighbouring heads go to neighbouring XCDs, except where two of them share a cache line (32 channels of 16 bits: 320 us one by one, 293
   // in pairs for 64 x 2000 rows of 32 heads; pairs of 64 channels: 230 against 225).
-  const int unit = HD * (int)sizeof(T) < 128 ? (turn >> 1) * 16 + (blockIdx.x & 7) * 2 + (turn & 1) : turn * 8 + (blockIdx.x & 7);
+  const int unit = W * (int)sizeof(T) < 128 ? (turn >> 1) * 16 + (blockIdx.x & 7) * 2 + (turn & 1) : turn * 8 + (blockIdx.x & 7);
   const int of = nr == 1 ? in : nr == 2 ? in >> 1 : in * 21846 >> 16;         // in / nr (in < 3 * 4096)
-  const int slot0 = unit / a.HK, hk = unit - slot0 * a.HK, h = hk * a.rep + of;
+  const int per = a.HK / HEADS, slot0 = unit / per, hk0 = (unit - slot0 * per) * HEADS, hk = hk0 + me, h0 = hk0 * a.rep + of, h = hk * a.rep + of;
   if (slot0 >= a.slots) return;
   const LinRole r = a.r[in - of * nr];                           // by value: its fields in a few wide loads, not one by one where they are used
   // the main kernel of a split axis starts with the last segments: their k and v are what the state kernel has read last
   const int slot = !STATE && a.split ? a.slots - 1 - slot0 : slot0;
-  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, n0 = (tid >> 6) * 16;
   // which score tiles this wave forms: the first of three waves changes from workgroup to workgroup (a wave stays on its SIMD)
-  const int mine_p = (__builtin_amdgcn_readfirstlane(tid >> 6) + blockIdx.y) % WAVES;
+  const int mine_p = (wi + blockIdx.y) % WAVES;
   LinSeq s;
   const bool mine = lin_find(a, slot, s);
   char* const out = (char*)r.o.p + h * r.o.h;
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       const int c0 = lin_cu(a, 0), cB = lin_cu(a, a.B), behind = slot - (cB / a.seg + a.B);
       if (behind >= 0) { z0 = cB + behind * a.seg; z1 = z0 + a.seg < a.T ? z0 + a.seg : a.T; }
       else if (slot <= c0 / a.seg) { z0 = slot * a.seg; z1 = z0 + a.seg < c0 ? z0 + a.seg : c0; }
-      for (long long i = tid; i < (long long)(z1 - z0) * HD; i += THREADS) {
+      for (long long i = tid - me * (HD * 4); i < (long long)(z1 - z0) * HD; i += HD * 4) {
         char* const at = out + (z0 + i / HD) * r.o.s;
         if (r.o32) ((float*)at)[i % HD] = 0.f; else ((T*)at)[i % HD] = (T)0.f;
       }
@@ -285,27 +288,28 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   const int row0 = rev ? s.begin + s.len - 1 : s.begin, dir = rev ? -1 : 1;        // row of position t: row0 + dir * t
   const int low = rev ? row0 - from - (C - 1) : row0 + from;
   const long long qs = r.q.s, ks = r.k.s, vs = r.v.s, os = r.o.s, n = a.cu ? 0 : b;
-  const char* bq = r.q.p + n * r.q.n + (r.shared & 1 ? hk : h) * r.q.h + low * qs;
-  const char* bk = r.k.p + n * r.k.n + (r.shared & 2 ? hk : h) * r.k.h + low * ks;
-  const char* bv = r.v.p + n * r.v.n + (r.shared & 4 ? hk : h) * r.v.h + low * vs;
-  char* bo = out + n * r.o.n + low * os;
+  const char* bq = r.q.p + n * r.q.n + (r.shared & 1 ? hk0 : h0) * r.q.h + low * qs;
+  const char* bk = r.k.p + n * r.k.n + (r.shared & 2 ? hk0 : h0) * r.k.h + low * ks;
+  const char* bv = r.v.p + n * r.v.n + (r.shared & 4 ? hk0 : h0) * r.v.h + low * vs;
+  char* bo = (char*)r.o.p + h0 * r.o.h + n * r.o.n + low * os;
   const long long dq = qs * (dir * C), dk = ks * (dir * C), dv = vs * (dir * C), dO = os * (dir * C);
   const bool o32 = r.o32;
   lin_raw pq[NU], pk[NU], pv[NU];                                // the next chunk's tiles, in flight during this one's math
   unsigned aq[NU], ak[NU], av[NU], ao[NU];
-  auto offsets = [&](unsigned (&off)[NU], long long stride, int c, bool in) __attribute__((always_inline)) {
+  auto offsets = [&](unsigned (&off)[NU], long long stride, unsigned head, int c, bool in) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int at = tid + u * THREADS, i = at / CPR < c ? at / CPR : c - 1;
-      off[u] = (unsigned)(rev ? c - 1 - i : i) * (unsigned)stride + ((at % CPR) ^ (in && DMA ? Tile::swz(at / CPR) : 0)) * 16;
+      const int piece = (at % CPR) ^ (in && DMA ? Tile::swz(at / CPR) : 0);
+      off[u] = (unsigned)(rev ? c - 1 - i : i) * (unsigned)stride + (HEADS == 1 ? 0 : piece / CPH * head) + piece % CPH * 16;
     }
   };
   auto offsets_in = [&](int c) __attribute__((always_inline)) {
-    if constexpr (!STATE) offsets(aq, qs, c, true);
-    offsets(ak, ks, c, true);
-    offsets(av, vs, c, true);
+    if constexpr (!STATE) offsets(aq, qs, (unsigned)r.q.h, c, true);
+    offsets(ak, ks, (unsigned)r.k.h, c, true);
+    offsets(av, vs, (unsigned)r.v.h, c, true);
   };
-  const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)sm + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+  const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)sm + wave * 1024;
   auto fetch = [&](int c, int stage) __attribute__((always_inline)) {
     if (c < C) {
       offsets_in(c);
@@ -339,10 +343,10 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   if constexpr (!STATE) {                                        // the first queries' weights of the second tile of keys are zeros for good
 #pragma unroll
     for (int k = 0; k < L::MID; ++k)
-      if (tid < 64) *(lin_half*)(sP + k * PPART + fr * PP + 16 * g + 8) = (lin_half){0u, 0u};
+      if (wi == 0) *(lin_half*)(sP + k * PPART + fr * PP + 16 * g + 8) = (lin_half){0u, 0u};
   }
   offsets_in(C);
-  if constexpr (!STATE) offsets(ao, os, C, false);
+  if constexpr (!STATE) offsets(ao, os, (unsigned)r.o.h, C, false);
   auto rows_at = [&](int t) __attribute__((always_inline)) { return upto - t < C ? upto - t : C; };
   if (from < upto) fetch(rows_at(from), 0);
 
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
         const float* const w = r.ws + ((long long)(s.np > LIN_INLINE ? slot : slot - s.p + p0 - u - 1) * a.H + h) * HD * HD;
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
-          if (!r.ws_t) x[u][t] = *(const f32x4*)(w + (((tid >> 6) * ND + t) * 64 + lane) * 4);
+          if (!r.ws_t) x[u][t] = *(const f32x4*)(w + ((wi * ND + t) * 64 + lane) * 4);
           else {                                                 // element (row, column) = (c, d) of the role that left it
             const int c = n0 + fr, d = lin_channel(t, g, 0), tile = 2 * (c >> 5) + (c >> 2 & 1);
 #pragma unroll
@@ -424,7 +428,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
     if constexpr (!STATE) {
       constexpr bool HOLD = L::IN == 1 && HD <= 64;              // else read again where they are used: too many registers
       lb8 qf[2][NK][L::IN];
-      auto query = [&](int ti, int kd) __attribute__((always_inline)) { Tile::row(sQ, ti, fr, kd, g, qf[ti][kd]); };
+      auto query = [&](int ti, int kd) __attribute__((always_inline)) { Tile::row(sQ, ti, fr, u0 + 8 * kd + 2 * g, qf[ti][kd]); };
       if constexpr (HOLD)
 #pragma unroll
         for (int kd = 0; kd < 2 * NK; ++kd) query(kd & 1, kd >> 1);
@@ -437,7 +441,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 #pragma unroll
           for (int kd = 0; kd < NK; ++kd) {
             lb8 kf[L::IN];
-            Tile::row(sK, e, fr, kd, g, kf);
+            Tile::row(sK, e, fr, u0 + 8 * kd + 2 * g, kf);
             if constexpr (!HOLD) query(ti, kd);
             p = lin_mma(kf, qf[ti][kd], p);
           }
@@ -462,7 +466,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       acc[1] *= lrow * l16;
     }
     lb8 vf[L::IN];
-    Tile::col_values(sV, n0, lane, vf);
+    Tile::col(sV, u0 + n0 / 4, 1, lane, vf);                     // column n0 + fr
     if (!END || !ends || r.last) {
       const int e = END && ends ? c - off : C;                   // the state behind the last row itself, or as the next row sees it
       const float le = END ? lin_pow(l2, e) : lC;
@@ -487,7 +491,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
         lb8 kf[L::IN];
-        Tile::col_state(sK, t, lane, kf);
+        Tile::col(sK, u0 + 8 * (t >> 1) + (t & 1), 2, lane, kf); // the columns lin_channel(t, ., .)
         S[t] = lin_mma(kf, p, S[t]);
       }
     }
@@ -504,7 +508,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
     if constexpr (!STATE) {
 #pragma unroll
       for (int ti = 0; ti < 2; ++ti) {
-        if (!o32) lin_store4((T*)(sO + (Tile::IN == 1 ? 16 * ti * OP + Tile::at(fr, n0 / 4 + g) : (16 * ti + fr) * OP + (n0 + 4 * g) * 4)), acc[ti]);
+        if (!o32) lin_store4((T*)(sO + (Tile::IN == 1 ? 16 * ti * OP + Tile::at(fr, u0 + n0 / 4 + g) : (16 * ti + fr) * OP + (n0 + 4 * g) * 4)), acc[ti]);
         else {
           const int t = t0 + 16 * ti + fr;
           if (t < upto) *(f32x4*)(out + n * r.o.n + (long long)(row0 + dir * t) * os + (n0 + 4 * g) * 4) = acc[ti];
@@ -517,7 +521,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
       // operands need: 2 to 5 % on every long case.
       if (!o32) {
         if (END && c < C) {
-          offsets(ao, os, c, false);
+          offsets(ao, os, (unsigned)r.o.h, c, false);
           if (rev) bo += (C - c) * os;
         }
 #pragma unroll
@@ -536,7 +540,7 @@ __global__ __launch_bounds__(HD * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) v
   }
   if (t0 < upto) chunk(std::true_type{}, t0, upto - t0, stage);
   if constexpr (STATE) {
-    f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + (tid >> 6) * ND * 64 + lane;
+    f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + wi * ND * 64 + lane;
 #pragma unroll
     for (int t = 0; t < ND; ++t) w[t * 64] = S[t];
   } else if (ends && r.last) {
@@ -705,18 +709,38 @@ static bool lin_tensor_ok(const void* p, const long long* st, int es) {
          st[1] * es < (1 << 26);                                 // (offsets inside a chunk are 32 bits)
 }
 
-static dim3 lin_grid(const LinArgs& a, int roles) {
-  const unsigned groups = (unsigned)(((long long)a.slots * a.HK + 15) / 16 * 2);       // (of eight, in pairs)
+static dim3 lin_grid(const LinArgs& a, int roles, int heads) {
+  const unsigned groups = (unsigned)(((long long)a.slots * (a.HK / heads) + 15) / 16 * 2);       // (of eight, in pairs)
   return dim3(8 * roles * a.rep, groups < LIN_GRID_Y ? groups : LIN_GRID_Y, (groups + LIN_GRID_Y - 1) / LIN_GRID_Y);
+}
+template <typename T, int HD, int HEADS, bool EXACT>
+static void lin_launch_heads(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
+  const dim3 block(HD * HEADS * 4);
+  if (p.split) {
+    hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, true, EXACT>), lin_grid(a, a.roles_state, HEADS), block, 0, stream, a);
+    if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)a.H * (HD * HD / 256) * (a.B < LIN_SCANS ? a.B : LIN_SCANS), a.roles_state), dim3(256), 0, stream, a, HD * HD);
+  }
+  hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, false, EXACT>), lin_grid(a, a.roles, HEADS), block, 0, stream, a);
+}
+// A head's 16-bit row is 64 or 128 bytes.  Four or two neighbouring heads to a workgroup read and write 256 at a time, which is worth more to
+// the memory than the larger workgroup costs, except where the card is not full of them or the kernel waits for its own steps:
+//   64 channels   64 x 2000 rows 212 us against 228, one recording 302 against 326; but 48 x 2000 rows (384 workgroups) 173 against 165, one clip
+//                 18.8 against 16.4, the training pair of 140-row clips 168 against 161, packed shared heads 120 against 101
+//   32 channels   64 x 2000 rows 210 us against 299, the training pairs of 140-row clips 152 against 172 and of 4 x 11025 rows 329 against 455;
+//                 of 2 x 2000 rows 49 against 47
+static bool lin_wide(const LinArgs& a, int HD, int heads) {
+  if (heads == 1 || a.HK % heads || a.rep > 1 || (HD > 32 && a.roles > 1)) return false;
+  if ((long long)a.slots * a.HK / heads < (HD > 32 ? LIN_WGS / 2 : LIN_WGS / 4)) return false;
+  for (int i = 0; i < a.roles; ++i)
+    for (const LinOperand* o : {&a.r[i].q, &a.r[i].k, &a.r[i].v, &a.r[i].o})
+      if (o->h < 0 || o->h >= (1 << 26)) return false;           // (offsets inside a chunk are 32 bits)
+  return true;
 }
 template <typename T, int HD, bool EXACT>
 static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
-  const dim3 block(HD * 4);
-  if (p.split) {
-    hipLaunchKernelGGL((lin_kernel<T, HD, true, EXACT>), lin_grid(a, a.roles_state), block, 0, stream, a);
-    if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)a.H * (HD * HD / 256) * (a.B < LIN_SCANS ? a.B : LIN_SCANS), a.roles_state), dim3(256), 0, stream, a, HD * HD);
-  }
-  hipLaunchKernelGGL((lin_kernel<T, HD, false, EXACT>), lin_grid(a, a.roles), block, 0, stream, a);
+  constexpr int HEADS = LinT<T>::IN == 1 ? 128 / HD : 1;
+  if (lin_wide(a, HD, HEADS)) lin_launch_heads<T, HD, HEADS, EXACT>(a, p, stream);
+  else lin_launch_heads<T, HD, 1, EXACT>(a, p, stream);
 }
 template <typename T, bool EXACT>
 static void lin_launch_t(const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {

@@ -426,6 +426,51 @@ def test_linear_attention_split_over_the_axis(ops, B, S, H, HK, HD, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("B,S,H,HD", [(64, 70, 16, 64), (34, 65, 32, 64), (64, 33, 16, 32), (256, 1, 4, 32)])
+def test_neighbouring_heads_in_one_workgroup(ops, B, S, H, HD):
+    """enough (sequence, head) pairs to give a workgroup two or four heads: the bits of the sequences one by one, and right ones"""
+    q, k, v, do, st, ds = lin_case(B, S, H, H, HD, torch.bfloat16, seed=5)
+    sl, scale = alibi(H), HD ** -0.5
+    d = [t.cuda() for t in (q, k, v, do, st, ds)]
+    got = (*ops.linear_attention_fwd(d[0], d[1], d[2], sl.cuda(), state=d[4], want_state=True),
+           *ops.linear_attention_bwd(d[0], d[1], d[2], sl.cuda(), d[3], state=d[4], d_state=d[5]))
+    for b in range(B):
+        one = [t[b:b + 1] for t in d]
+        want = (*ops.linear_attention_fwd(one[0], one[1], one[2], sl.cuda(), state=one[4].contiguous(), want_state=True),
+                *ops.linear_attention_bwd(one[0], one[1], one[2], sl.cuda(), one[3], state=one[4].contiguous(), d_state=one[5].contiguous()))
+        for x, y in zip(got, want):
+            assert torch.equal(x[b], y[0])
+    lin_check([t[:2] for t in got], [(q[b], k[b], v[b], do[b], st[b], ds[b]) for b in range(2)], sl, scale, torch.bfloat16, H, H, HD)
+
+
+@gpu
+@pytest.mark.parametrize("H,HD,far", [(32, 64, False), (32, 32, False), (2, 64, True)])
+def test_neighbouring_heads_of_a_long_recording(ops, H, HD, far):
+    """the same of a split axis, with rows outside the sequence, from a packed projection; heads too far apart for it take the other kernel"""
+    S, lead, tail = (524320, 0, 0) if far else (40000, 40, 1000)
+    cu = torch.tensor([lead, S - tail], dtype=torch.int32, device="cuda")
+    sl = (alibi(H) + 0.5).cuda()
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.randn(1, 3, H, S, HD, generator=g, device="cuda").to(torch.bfloat16)
+    q, k, v = x.transpose(2, 3).unbind(1)
+    if not far:
+        q, k, v = x.permute(0, 3, 1, 2, 4).contiguous().unbind(2)
+    out, last = ops.linear_attention_fwd(q, k, v, sl, cu_seqlens=cu, want_state=True)
+    n = [t[0, S - tail - 300:S - tail].double().cpu() for t in (q, k, v)]     # e^(-0.5 * 200): what lies further back is below every rounding
+    want = ref_linear(*n, sl.cpu(), HD ** -0.5)
+    size = ref_linear(*(t.abs() for t in n), sl.cpu(), HD ** -0.5)
+    check(out[0, S - tail - 100:S - tail], want[0][-100:], size[0][-100:] + 1.0, 2.0 ** -14, "last rows")
+    check(last[0], want[1], size[1], c_of(torch.float32, 300, HD), "state")
+    assert not out[0, :lead].any() and not out[0, S - tail:].any()
+    dense, _ = ops.linear_attention_fwd(*(t[:, lead:S - tail].contiguous() for t in (q, k, v)), sl)
+    n = [t[0, lead:lead + 200].double().cpu() for t in (q, k, v)]
+    want = ref_linear(*n, sl.cpu(), HD ** -0.5)
+    size = ref_linear(*(t.abs() for t in n), sl.cpu(), HD ** -0.5)
+    for t in (out[0, lead:lead + 200], dense[0, :200]):
+        check(t, want[0], size[0], 2.0 ** -14, "first rows")
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("lens,lead,tail,H,HK,HD", [((5, 0, 64, 1, 130, 0), 3, 9, 4, 2, 64), ((0,), 0, 4, 2, 2, 32), ((700, 3, 0, 1200, 256), 17, 300, 2, 1, 32), ((40, 90), 0, 0, 2, 2, 128)])
 def test_linear_attention_packed(ops, lens, lead, tail, H, HK, HD, dtype):
