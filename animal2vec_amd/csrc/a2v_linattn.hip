@@ -415,10 +415,9 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
     const char* const sV = sK + Tile::BYTES;
     const char* const sQ = sK + (STATE ? 0 : 2) * Tile::BYTES;
     if constexpr (DMA) {
-      // Younger than this chunk's loads are the rows that the last chunk has stored.  Where every operand is read by one workgroup, memory is
-      // what bounds the kernel, and it is faster if a workgroup's stores are through before it goes on (64 x 2000 rows: 229 us against 240);
-      // where roles or shared heads meet in the L2 it is not (training pair of 140 rows 161 against 156, ragged shared heads 108 against 103).
-      if (END || STATE || o32 || t0 == from || a.roles * a.rep == 1) lin_wait<0>();
+      // Younger than this chunk's loads are the rows that the last chunk has stored; nothing waits for them.  (Waiting is 1 % faster where memory
+      // binds and the card is full, and up to 13 % slower elsewhere: 16 x 2000 rows of 32 heads of 32 channels 85 us against 74.)
+      if (END || STATE || o32 || t0 == from) lin_wait<0>();
       else lin_wait<NU>();
     } else place();
     __syncthreads();
@@ -725,7 +724,8 @@ static void lin_launch_heads(const LinArgs& a, const LinPlan& p, hipStream_t str
 // A head's 16-bit row is 64 or 128 bytes.  Four or two neighbouring heads to a workgroup read and write 256 at a time, which is worth more to
 // the memory than the larger workgroup costs, except where the card is not full of them or the kernel waits for its own steps:
 //   64 channels   64 x 2000 rows 212 us against 228, one recording 302 against 326; but 48 x 2000 rows (384 workgroups) 173 against 165, one clip
-//                 18.8 against 16.4, the training pair of 140-row clips 168 against 161, packed shared heads 120 against 101
+//                 18.8 against 16.4, the training pair of 140-row clips 168 against 161 (its forward alone 50 against 48), packed shared heads 120
+//                 against 101
 //   32 channels   64 x 2000 rows 210 us against 299, the training pairs of 140-row clips 152 against 172 and of 4 x 11025 rows 329 against 455;
 //                 of 2 x 2000 rows 49 against 47
 static bool lin_wide(const LinArgs& a, int HD, int heads) {
