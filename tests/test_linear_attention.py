@@ -777,6 +777,29 @@ def test_calls_on_two_streams_and_from_two_threads(ops):
 
 
 @gpu
+@pytest.mark.parametrize("N,H,HD", [(64, 16, 64), (2, 16, 64), (3, 2, 128)])
+def test_rows_far_apart(ops, N, H, HD):
+    """rows 60 MiB apart: offsets inside a chunk pass 31 bits; results in such rows as well, and the bytes between them left alone"""
+    S, row = 33, 30 << 20
+    base = torch.zeros((S - 1) * row + 4 * N * H * HD, dtype=torch.bfloat16, device="cuda")
+    view = lambda i: base.as_strided((N, S, H, HD), (4 * H * HD, row, HD, 1), i * H * HD)          # noqa: E731
+    q, k, v, out = (view(i) for i in range(4))
+    g = torch.Generator("cuda").manual_seed(1)
+    for t in (q, k, v):
+        t.copy_(torch.randn(N, S, H, HD, generator=g, device="cuda"))
+    sl = alibi(H).cuda()
+    want, _ = ops.linear_attention_fwd(q.contiguous(), k.contiguous(), v.contiguous(), sl)
+    kept = [t.clone() for t in (q, k, v)]
+    ops.linear_attention_fwd(q, k, v, sl, out=out)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(kept, (q, k, v)))
+    assert not base[4 * N * H * HD:row].any()
+    do = rnd(N, S, H, HD, seed=4, dtype=torch.bfloat16).cuda()
+    grads = ops.linear_attention_bwd(*(t.contiguous() for t in (q, k, v)), sl, do)
+    for a, b in zip(grads[:3], ops.linear_attention_bwd(q, k, v, sl, do)):
+        assert torch.equal(a, b)
+
+
+@gpu
 def test_long_offsets_pass_32_bits(ops):
     """a packed buffer of more than 2^31 elements: the last rows are as right as the first ones (addresses are formed in 64 bits)"""
     H, HD, W = 2, 64, 60 * 64
