@@ -567,7 +567,7 @@ def rope_inv_freq(sections, base=10000.0, device="cuda"):
 
 # A call's checks, strides and sizes depend on layouts alone (shapes, strides, types, devices, options): they are worked out once per
 # layout, so that the next frame of a stream pays for a dictionary look-up.  Nothing of the tensors themselves is kept; what depends on
-# addresses (alignment, overlap) is checked in every call.
+# addresses (alignment, overlap) is checked in every call (overlap of views of one buffer: by where they lie relative to each other).
 _LAYOUTS = {}
 
 
@@ -687,6 +687,28 @@ def _apart(what, outs, ins, inplace=False):
             raise ValueError(f"{what}: two outputs overlap")
 
 
+def _spans(outs, ins):
+    """what _apart_again needs of a layout: the bytes that each tensor reaches over, and the relative positions found to be apart"""
+    return [(sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0 for t in (*outs, *ins)], set()
+
+
+def _apart_again(what, spans, outs, ins, inplace=False):
+    """_apart for another call of one layout: tensors whose ranges of addresses meet are looked at once for each of their relative positions"""
+    ext, seen = spans
+    ps = [t.data_ptr() for t in (*outs, *ins)]
+    for i in range(len(outs)):
+        p, e = ps[i], ps[i] + ext[i]
+        for j in range(i + 1, len(ps)):
+            if ps[j] < e and p < ps[j] + ext[j]:
+                at = tuple(x - p for x in ps)
+                if (i, at) not in seen:
+                    _apart(what, outs, ins, inplace)
+                    if len(seen) >= 64:
+                        seen.clear()
+                    seen.add((i, at))
+                return
+
+
 def _strides(*ts):
     """(sequence, row, head) strides of each tensor as a host array (a dimension of one row counts as 0: it is never stepped along)"""
     return (C.c_longlong * (3 * len(ts)))(*[s if n > 1 else 0 for t in ts for s, n in zip(t.stride()[:3], t.shape)])
@@ -745,10 +767,10 @@ def qk_norm_rope_fwd(q, k, q_weight, k_weight, inv_freq, pos=None, *, sections=N
             _apart(what, (q_out, k_out), (q, k), inplace=True)         # (before the device check: a refusal does not depend on the device)
         _starts(what, q, k, q_out, k_out, q_weight, k_weight)
         _on_gpu(q)
-        return (_strides(q, k, q_out, k_out), *p)
-    st, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections), (q, k, q_weight, k_weight, inv_freq, pos, *((q_out, k_out) if given else ())), plan)
+        return (_spans((q_out, k_out), (q, k)), _strides(q, k, q_out, k_out), *p)
+    spans, st, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections), (q, k, q_weight, k_weight, inv_freq, pos, *((q_out, k_out) if given else ())), plan)
     if given:
-        _apart(what, (q_out, k_out), (q, k), inplace=True)
+        _apart_again(what, spans, (q_out, k_out), (q, k), inplace=True)
     if q.numel() == 0:
         return q_out, k_out
     _run(_L().a2v_qk_norm_rope_fwd, "a2v_qk_norm_rope_fwd", q.device, code, *_starts(what, q, k, q_out, k_out), st, *_starts(what, q_weight, k_weight),
@@ -779,13 +801,13 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, inv_freq, pos=Non
             _apart(what, (dq, dk), (dq_out, dk_out, q, k), inplace=True)
         _starts(what, dq_out, dk_out, q, k, dq, dk, q_weight, k_weight)
         _on_gpu(q)
-        return (_strides(dq_out, dk_out, q, k, dq, dk), _L().a2v_qk_norm_rope_workspace(*p[-1]), *p)
-    st, need, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections),
+        return (_spans((dq, dk), (dq_out, dk_out, q, k)), _strides(dq_out, dk_out, q, k, dq, dk), _L().a2v_qk_norm_rope_workspace(*p[-1]), *p)
+    spans, st, need, code, ps, axes, sec, sizes = _layout(what, None if sections is None else tuple(sections),
                                                    (q, k, q_weight, k_weight, inv_freq, pos, dq_out, dk_out, dq_weight, dk_weight, *((dq, dk) if given else ())), plan)
     if abs(dq_weight.data_ptr() - dk_weight.data_ptr()) < 4 * q.shape[3]:
         raise ValueError(f"{what}: dq_weight and dk_weight must be two buffers (both are accumulated at once)")
     if given:
-        _apart(what, (dq, dk), (dq_out, dk_out, q, k), inplace=True)
+        _apart_again(what, spans, (dq, dk), (dq_out, dk_out, q, k), inplace=True)
     if q.numel() == 0:
         return dq, dk
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -836,10 +858,10 @@ def linear_attention_fwd(q, k, v, slopes, *, scale=None, state=None, cu_seqlens=
             _apart(what, (out,), (q, k, v))
         _starts(what, q, k, v, out)
         _on_gpu(q)
-        return dt(q), _strides(q, k, v, out), sizes, _L().a2v_linear_attention_workspace(dt(q), 0, cu_seqlens is not None, *sizes)
-    code, st, sizes, need = _layout(what, None, (q, k, v, slopes, state, cu_seqlens, out if given else None), plan)
+        return _spans((out,), (q, k, v)), dt(q), _strides(q, k, v, out), sizes, _L().a2v_linear_attention_workspace(dt(q), 0, cu_seqlens is not None, *sizes)
+    spans, code, st, sizes, need = _layout(what, None, (q, k, v, slopes, state, cu_seqlens, out if given else None), plan)
     if given:
-        _apart(what, (out,), (q, k, v))
+        _apart_again(what, spans, (out,), (q, k, v))
     B, _, H, _, HD = sizes
     last = torch.empty((B, H, HD, HD), dtype=torch.float32, device=q.device) if want_state else None
     if B == 0:
@@ -872,10 +894,10 @@ def linear_attention_bwd(q, k, v, slopes, d_out, *, scale=None, state=None, d_st
             _apart(what, (dq, dk, dv), (q, k, v, d_out))
         _starts(what, q, k, v, d_out, dq, dk, dv)
         _on_gpu(q)
-        return dt(q), _strides(q, k, v, d_out, dq, dk, dv), sizes, _L().a2v_linear_attention_workspace(dt(q), 1, cu_seqlens is not None, *sizes)
-    code, st, sizes, need = _layout(what, None, (q, k, v, slopes, d_out, state, d_state, cu_seqlens, *((dq, dk, dv) if given else ())), plan)
+        return _spans((dq, dk, dv), (q, k, v, d_out)), dt(q), _strides(q, k, v, d_out, dq, dk, dv), sizes, _L().a2v_linear_attention_workspace(dt(q), 1, cu_seqlens is not None, *sizes)
+    spans, code, st, sizes, need = _layout(what, None, (q, k, v, slopes, d_out, state, d_state, cu_seqlens, *((dq, dk, dv) if given else ())), plan)
     if given:
-        _apart(what, (dq, dk, dv), (q, k, v, d_out))
+        _apart_again(what, spans, (dq, dk, dv), (q, k, v, d_out))
     first = None if state is None else torch.empty_like(state)
     if sizes[0] == 0:
         return dq, dk, dv, first
@@ -916,10 +938,10 @@ def linear_attention_step(q, k, v, slopes, state, *, slots=None, scale=None, out
         _starts(what, q, k, v, out)
         _on_gpu(q)
         st = (C.c_longlong * 8)(*[s if n > 1 else 0 for t in (q, k, v, out) for s, n in zip(t.stride()[:2], t.shape)])
-        return dt(q), st, (state.shape[0], N, H, k.shape[1], HD, HD ** -0.5)
-    code, st, sizes = _layout(what, None, (q, k, v, slopes, state, slots, out if given else None), plan)
+        return _spans((out,), (q, k, v)), dt(q), st, (state.shape[0], N, H, k.shape[1], HD, HD ** -0.5)
+    spans, code, st, sizes = _layout(what, None, (q, k, v, slopes, state, slots, out if given else None), plan)
     if given:
-        _apart(what, (out,), (q, k, v))
+        _apart_again(what, spans, (out,), (q, k, v))
     if sizes[1] == 0:
         return out
     if scale is not None:

@@ -140,6 +140,30 @@ def test_norm_rope_refusals(change):
         ops.qk_norm_rope_fwd(**{**_rope_args(), **change})
 
 
+def test_overlap_of_a_layout_seen_before():
+    """a layout's verdict holds for the relative positions it was found at, not for others"""
+    from animal2vec_amd import ops
+    buf = torch.zeros(4096, dtype=torch.bfloat16)
+    t = lambda at: buf.as_strided((1, 4, 2, 64), (512, 128, 64, 1), at)        # noqa: E731
+    a, b, far, onto = t(0), t(512), t(2048), t(64)
+    rows = buf.view(1, 8, 8, 64)
+    spans = ops._spans((a, b), (a, b))
+    for _ in range(2):
+        ops._apart_again("x", spans, (a, b), (a, b), inplace=True)
+        ops._apart_again("x", spans, (a, b), (far, t(2560)), inplace=True)
+        for bad in (((a, b), (b, a)), ((a, onto), (a, b)), ((a, b), (far, onto)), ((a, a), (far, b))):
+            with pytest.raises(ValueError, match="overlap"):
+                ops._apart_again("x", spans, *bad, inplace=True)
+    # slots of one packed buffer meet in their ranges and are apart; moved by a head they are not
+    q, k, v, o = (rows[:, :, i:i + 2] for i in (0, 2, 4, 6))
+    spans = ops._spans((o,), (q, k, v))
+    for _ in range(2):
+        ops._apart_again("x", spans, (o,), (q, k, v))
+        ops._apart_again("x", spans, (q,), (k, v, o))
+        with pytest.raises(ValueError, match="overlap"):
+            ops._apart_again("x", spans, (rows[:, :, 5:7],), (q, k, v))
+
+
 def test_outputs_may_not_overlap():
     from animal2vec_amd import ops
     qkv = torch.zeros(2, 5, 3, 4, 64, dtype=torch.bfloat16)
