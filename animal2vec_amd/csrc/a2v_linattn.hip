@@ -20,8 +20,9 @@
 //
 // All products run on the bf16 matrix cores, fp32 values as sums of bf16 parts of 8 bits each (x = hi + mid + lo exactly; the products of
 // parts are exact in the fp32 accumulators):
-//   bf16 operands: q, k, v are one part; scores and the state two (2^-16 relative), the scaled values two, or three where the state is
-//     a result.  One rounding of each to 16 bits would add up to more than the one rounding of the result that the type asks for.
+//   bf16 operands: q, k, v are one part; scores, the state that rows read and the scaled values that it sums are three, all of their 32 bits.
+//     (Two parts, 2^-16 relative, turn over one rounding in 1000 of the results and are 6 % faster: 64 clips of 2000 rows 214 us against 218, the
+//     training pair of 140-row clips 156 against 181.)
 //   fp32 operands: three parts of everything, six products of parts (the three below 2^-24 are dropped): 96 matrix cycles for 32 channels
 //     of a 16 x 16 tile where v_mfma_f32_16x16x4_f32 takes 256.
 #include "a2v_common.h"
@@ -69,8 +70,9 @@ struct LinArgs {
 // of 128: 3 workgroups on a CU, not 4 (64 clips of 2000 rows 11 % slower, the training pair of 140-row clips 24 %).
 #define LIN_C 32
 template <typename T> struct LinT;
-template <> struct LinT<__bf16> { static constexpr int IN = 1, MID = 2, V = 8; };      // parts of the operands, of scores and states; elements of 16 bytes
-template <> struct LinT<float> { static constexpr int IN = 3, MID = 3, V = 4; };
+template <> struct LinT<__bf16> { static constexpr int IN = 1, V = 8; };               // parts of the operands; elements of 16 bytes
+template <> struct LinT<float> { static constexpr int IN = 3, V = 4; };
+#define LIN_MID 3             /* parts of scores, scaled values and states: all of 32 bits */
 
 // x[0 .. 2 N - 1] = the sum of PARTS bf16 parts: the nearest, the nearest to what is left, and so on; two elements at a time (v_cvt_pk,
 // then a shift and a mask to get the pair back: 6 instructions a pair and part)
@@ -218,13 +220,12 @@ __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amd
 // a chain of LDS reads, matrix and vector steps of 2 us, and four waves to a SIMD do not hide all of it.  A recording reads k and v twice, and
 // a long backward's dq, which runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory
 // instead of 4.
-// Registers: 128 with 16-bit operands, four waves to a SIMD; three parts take 166, three waves (two: 90 us against 84 for the training pair
+// Registers: 128 with 16-bit operands, four waves to a SIMD; 32-bit ones take 166, three waves (two: 90 us against 84 for the training pair
 // of 2 x 2000 rows in fp32), with 128 channels two.
 //
 // HEADS: neighbouring heads of a workgroup (lin_wide), each with waves, scores and state of its own, side by side in the tiles' rows.
 // STATE: only the segment's own state (from zero) is formed, into ws: what the segments behind it start from.
-// EXACT: the state is a result (or might be: out does not depend on that) and keeps all of its 32 bits with a third part of the values.
-template <typename T, int HD, int HEADS, bool STATE, bool EXACT>
+template <typename T, int HD, int HEADS, bool STATE>
 __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 2 : 3) void lin_kernel(LinArgs a) {
   typedef LinT<T> L;
   constexpr int W = HD * HEADS;                                  // channels of a row of the tiles
@@ -232,16 +233,19 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
   constexpr int C = LIN_C, ND = HD / 16, NK = HD / 32, THREADS = W * 4, OP = Tile::IN == 1 ? 2 * W : 4 * W + 16;            // OP: pitch of the result's tile, bytes
   constexpr int CPH = HD / L::V, CPR = W / L::V, NU = C * CPR / THREADS;         // 16-byte pieces of a row, and of a tile for each thread
   static_assert(C * CPR == NU * THREADS, "whole pieces per thread and tile");
+  static_assert(L::IN > 1 || C * OP == Tile::BYTES, "the result takes the place of the queries");
   constexpr int WAVES = HD / 16, PP = 80, PPART = C * PP;        // scores: rows of 32 bf16 at a pitch of 20 words (16 rows, 16 lanes: all banks)
   // 16-bit operands go straight to LDS, into two stages of tiles in turn; 32-bit ones are split on the way, through registers.  (Two chunks
   // ahead instead of one: 0 to 3 % slower.)
   constexpr bool DMA = L::IN == 1;
   constexpr int LOADS = STATE ? 2 : 3, STAGE = LOADS * Tile::BYTES;
-  __shared__ __attribute__((aligned(16))) char sm[(DMA ? 2 : 1) * STAGE + (STATE ? 0 : C * OP + HEADS * L::MID * PPART)];
-  char* const sO = sm + (STATE ? 0 : (DMA ? 2 : 1) * STAGE);
+  // the result's tile: with two stages, over the chunk's queries, which are done with by then (four heads of 32 channels would not fit twice
+  // on a CU with one of its own)
+  constexpr int RES = STATE || DMA ? 0 : C * OP;
+  __shared__ __attribute__((aligned(16))) char sm[(DMA ? 2 : 1) * STAGE + RES + (STATE ? 0 : HEADS * LIN_MID * PPART)];
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int me = HEADS == 1 ? 0 : wave / WAVES, wi = wave - me * WAVES, n0 = wi * 16, u0 = me * (HD / 4);       // head of the workgroup, wave of the head
-  char* const sP = sO + (STATE ? 0 : C * OP + me * L::MID * PPART);
+  char* const sP = sm + (DMA ? 2 : 1) * STAGE + RES + (STATE ? 0 : me * LIN_MID * PPART);
   // Workgroups go to the eight XCDs in turn.  What reads the same rows at the same time -- the roles of a backward, the heads that share
   // k and v -- is put eight apart: one XCD, one L2.  (Side by side, the three roles of a backward read everything from memory three times.)
   const int nr = STATE ? a.roles_state : a.roles, in = blockIdx.x >> 3, turn = blockIdx.z * LIN_GRID_Y + blockIdx.y;
@@ -342,7 +346,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
 
   if constexpr (!STATE) {                                        // the first queries' weights of the second tile of keys are zeros for good
 #pragma unroll
-    for (int k = 0; k < L::MID; ++k)
+    for (int k = 0; k < LIN_MID; ++k)
       if (wi == 0) *(lin_half*)(sP + k * PPART + fr * PP + 16 * g + 8) = (lin_half){0u, 0u};
   }
   offsets_in(C);
@@ -414,6 +418,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
     const char* const sK = sm + stage;
     const char* const sV = sK + Tile::BYTES;
     const char* const sQ = sK + (STATE ? 0 : 2) * Tile::BYTES;
+    char* const sO = sm + (DMA ? stage + 2 * Tile::BYTES : STAGE);
     if constexpr (DMA) {
       // Younger than this chunk's loads are the rows that the last chunk has stored; nothing waits for them.  (Waiting is 1 % faster where memory
       // binds and the card is full, and up to 13 % slower elsewhere: 16 x 2000 rows of 32 heads of 32 channels 85 us against 74.)
@@ -425,7 +430,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
     f32x4 acc[2];                                                // results of the two query tiles
     acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if constexpr (!STATE) {
-      constexpr bool HOLD = L::IN == 1 && HD <= 64;              // else read again where they are used: too many registers
+      constexpr bool HOLD = L::IN == 1 && W <= 64;              // else read again where they are used: too many registers
       lb8 qf[2][NK][L::IN];
       auto query = [&](int ti, int kd) __attribute__((always_inline)) { Tile::row(sQ, ti, fr, u0 + 8 * kd + 2 * g, qf[ti][kd]); };
       if constexpr (HOLD)
@@ -448,15 +453,15 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
 #pragma unroll
           for (int i = 0; i < 4; ++i)                            // on the diagonal a select, not a product: a non-finite key stays behind
             x[i] = n == 1 ? p[i] * w1[i] : fr < 4 * g + i ? 0.f : p[i] * w0[i];
-          unsigned w[L::MID][2];
-          lin_split<L::MID, 2>(x, w);
+          unsigned w[LIN_MID][2];
+          lin_split<LIN_MID, 2>(x, w);
 #pragma unroll
-          for (int k = 0; k < L::MID; ++k) *(lin_half*)(sP + k * PPART + (16 * ti + fr) * PP + 16 * g + 8 * e) = (lin_half){w[k][0], w[k][1]};
+          for (int k = 0; k < LIN_MID; ++k) *(lin_half*)(sP + k * PPART + (16 * ti + fr) * PP + 16 * g + 8 * e) = (lin_half){w[k][0], w[k][1]};
         }
 #pragma unroll
       for (int kd = 0; kd < NK; ++kd) {
-        lb8 y[L::MID];
-        lin_split_tiles<L::MID>(S[2 * kd], S[2 * kd + 1], minus, y);
+        lb8 y[LIN_MID];
+        lin_split_tiles<LIN_MID>(S[2 * kd], S[2 * kd + 1], minus, y);
         if constexpr (!HOLD) { query(0, kd); query(1, kd); }
         acc[0] = lin_mma(y, qf[0][kd], acc[0]);
         acc[1] = lin_mma(y, qf[1][kd], acc[1]);
@@ -485,8 +490,8 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
           x[i >> 2][i & 3] = j < c ? lin_value(vf, i) * (r.s_state * lin_pow(l2, e - j)) : 0.f;     // (rows behind the end are copies of the last)
         }
       }
-      lb8 p[EXACT ? 3 : L::MID];
-      lin_split_tiles<EXACT ? 3 : L::MID>(x[0], x[1], minus, p);
+      lb8 p[LIN_MID];
+      lin_split_tiles<LIN_MID>(x[0], x[1], minus, p);
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
         lb8 kf[L::IN];
@@ -498,9 +503,9 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
     if constexpr (!STATE) {
 #pragma unroll
       for (int ti = 0; ti < 2; ++ti) {
-        lb8 p[L::MID];
+        lb8 p[LIN_MID];
 #pragma unroll
-        for (int k = 0; k < L::MID; ++k) p[k] = *(const lb8*)(sP + k * PPART + (16 * ti + fr) * PP + 16 * g);
+        for (int k = 0; k < LIN_MID; ++k) p[k] = *(const lb8*)(sP + k * PPART + (16 * ti + fr) * PP + 16 * g);
         acc[ti] = lin_mma(vf, p, acc[ti]);
       }
     }
@@ -712,14 +717,14 @@ static dim3 lin_grid(const LinArgs& a, int roles, int heads) {
   const unsigned groups = (unsigned)(((long long)a.slots * (a.HK / heads) + 15) / 16 * 2);       // (of eight, in pairs)
   return dim3(8 * roles * a.rep, groups < LIN_GRID_Y ? groups : LIN_GRID_Y, (groups + LIN_GRID_Y - 1) / LIN_GRID_Y);
 }
-template <typename T, int HD, int HEADS, bool EXACT>
+template <typename T, int HD, int HEADS>
 static void lin_launch_heads(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
   const dim3 block(HD * HEADS * 4);
   if (p.split) {
-    hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, true, EXACT>), lin_grid(a, a.roles_state, HEADS), block, 0, stream, a);
+    hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, true>), lin_grid(a, a.roles_state, HEADS), block, 0, stream, a);
     if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)a.H * (HD * HD / 256) * (a.B < LIN_SCANS ? a.B : LIN_SCANS), a.roles_state), dim3(256), 0, stream, a, HD * HD);
   }
-  hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, false, EXACT>), lin_grid(a, a.roles, HEADS), block, 0, stream, a);
+  hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, false>), lin_grid(a, a.roles, HEADS), block, 0, stream, a);
 }
 // A head's 16-bit row is 64 or 128 bytes.  Four or two neighbouring heads to a workgroup read and write 256 at a time, which is worth more to
 // the memory than the larger workgroup costs, except where the card is not full of them or the kernel waits for its own steps:
@@ -736,23 +741,21 @@ static bool lin_wide(const LinArgs& a, int HD, int heads) {
       if (o->h < 0 || o->h >= (1 << 26)) return false;           // (offsets inside a chunk are 32 bits)
   return true;
 }
-template <typename T, int HD, bool EXACT>
+template <typename T, int HD>
 static void lin_launch_hd(const LinArgs& a, const LinPlan& p, hipStream_t stream) {
   constexpr int HEADS = LinT<T>::IN == 1 ? 128 / HD : 1;
-  if (lin_wide(a, HD, HEADS)) lin_launch_heads<T, HD, HEADS, EXACT>(a, p, stream);
-  else lin_launch_heads<T, HD, 1, EXACT>(a, p, stream);
+  if (lin_wide(a, HD, HEADS)) lin_launch_heads<T, HD, HEADS>(a, p, stream);
+  else lin_launch_heads<T, HD, 1>(a, p, stream);
 }
-template <typename T, bool EXACT>
+template <typename T>
 static void lin_launch_t(const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {
-  if (HD == 32) lin_launch_hd<T, 32, EXACT>(a, p, stream);
-  else if (HD == 64) lin_launch_hd<T, 64, EXACT>(a, p, stream);
-  else lin_launch_hd<T, 128, EXACT>(a, p, stream);
+  if (HD == 32) lin_launch_hd<T, 32>(a, p, stream);
+  else if (HD == 64) lin_launch_hd<T, 64>(a, p, stream);
+  else lin_launch_hd<T, 128>(a, p, stream);
 }
-// exact: a state is a result, or might be
-static void lin_launch(int dtype, const LinArgs& a, const LinPlan& p, int HD, bool exact, hipStream_t stream) {
-  if (dtype == A2V_F32) lin_launch_t<float, false>(a, p, HD, stream);        // (three parts of everything as it is)
-  else if (exact) lin_launch_t<__bf16, true>(a, p, HD, stream);
-  else lin_launch_t<__bf16, false>(a, p, HD, stream);
+static void lin_launch(int dtype, const LinArgs& a, const LinPlan& p, int HD, hipStream_t stream) {
+  if (dtype == A2V_F32) lin_launch_t<float>(a, p, HD, stream);
+  else lin_launch_t<__bf16>(a, p, HD, stream);
 }
 static int lin_dtype(int dtype) {
   if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
@@ -795,7 +798,7 @@ extern "C" int a2v_linear_attention_fwd(int dtype, const void* q, const void* k,
                    kv, 0, 0, 0, 0, scale, 1.f, state, state_out, (float*)ws};
   a.r[1] = a.r[2] = a.r[0];
   a.roles = a.roles_state = 1;
-  lin_launch(dtype, a, p, HD, true, stream);
+  lin_launch(dtype, a, p, HD, stream);
   A2V_CHECK_LAUNCH();
   return A2V_OK;
 }
@@ -836,7 +839,7 @@ extern "C" int a2v_linear_attention_bwd(int dtype, const void* q, const void* k,
   a.r[1] = LinRole{K, Q, D, gv, kv, 1, 0, 0, o32, 1.f, scale, d_state_out, d_state, (float*)(w + p.states)};
   a.r[2] = LinRole{V, D, Q, gk, kv, 1, 1, 1, o32, 1.f, scale, d_state_out, nullptr, (float*)(w + p.states)};
   a.roles = 3; a.roles_state = 2;                                // dk's segment states are the transposes of dv's
-  lin_launch(dtype, a, p, HD, d_state != nullptr, stream);
+  lin_launch(dtype, a, p, HD, stream);
   if (rep > 1 && rows) {
     const dim3 grid((unsigned)cdiv((long)(rows * HK * HD / 4), 256));
     if (dtype == A2V_F32)

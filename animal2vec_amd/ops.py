@@ -845,7 +845,7 @@ def linear_attention_fwd(q, k, v, slopes, *, scale=None, state=None, cu_seqlens=
     scale: default HD^-0.5.  state (B,H,HD,HD) fp32: what the sequences start from (None: nothing), never changed.
     cu_seqlens (B+1) int32 on the device: q, k, v are (1,T,heads,HD) and sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1], which may
     be none; rows outside every sequence are zeros in a result of this call's own and left as they were in the caller's `out`.
-    The products take 16-bit operands as pairs: sums, scores and states keep fp32 accuracy, out is rounded once."""
+    Sums, scores and states keep fp32's bits in both types, out is rounded once."""
     what = "linear_attention_fwd"
     given = out is not None
     if not given:

@@ -1,0 +1,130 @@
+"""Linear attention where it can go wrong and random inputs do not show it: the bits of what is kept between the products, and what the
+tests beside these (test_linear_attention.py, whose references and bounds are used here) leave out."""
+import pytest
+import torch
+
+from test_linear_attention import U, alibi, c_of, check, lin_case, ref_linear, rnd
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    from animal2vec_amd import ops as o
+    return o
+
+
+# ------------------------------------------------------------------------------------------------ bits
+# Two terms of size A that are equal up to 2^-12 are subtracted: the result's own rounding, u 2^-12 A = 2^-20 A in bf16, is below what a
+# term loses if it is kept in 16 bits (up to 2^-16 A), and above what is lost in 32 (c A, c counted at each test).
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_keep_32_bits(ops, dtype):
+    """v is 1 and -1 in two rows whose scores are equal up to 2^-12.  A score: HD products added in 32 bits, its weight and scale 8 more
+    roundings: c = (HD + 8) 2^-24"""
+    B, H, HD = 64, 4, 32
+    q, k = rnd(B, 2, H, HD, seed=1, dtype=dtype), rnd(B, 2, H, HD, seed=2, dtype=dtype).abs()
+    q = q.abs() + torch.tensor(0.5, dtype=dtype)
+    k[:, 1] = k[:, 0]
+    k[:, 0, :, 0], k[:, 1, :, 0] = 2.0 ** -8, 0.0            # q_0 2^-8 of about 20
+    v = torch.zeros(B, 2, H, HD, dtype=dtype)
+    v[:, 0], v[:, 1] = 1.0, -1.0
+    sl = torch.zeros(H)
+    out, _ = ops.linear_attention_fwd(q.cuda(), k.cuda(), v.cuda(), sl.cuda())
+    for b in range(B):
+        want = ref_linear(q[b].double(), k[b].double(), v[b].double(), sl, HD ** -0.5)[0]
+        size = ref_linear(q[b].double(), k[b].double(), v[b].double().abs(), sl, HD ** -0.5)[0]
+        assert float((want[1].abs() / size[1]).max()) < 2.0 ** -10
+        check(out[b], want, size, (HD + 8) * 2.0 ** -24, f"sequence {b}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,HD,B", [(4, 32, 8), (2, 64, 8), (2, 128, 8), (16, 64, 64)])
+def test_the_state_that_rows_read_keeps_32_bits(ops, dtype, H, HD, B):
+    """a row with q = (1, -1, 0 ...) and no key reads the difference of two rows of the state.  Decay, scale and sum of two terms: 8
+    roundings.  Forward (out) and backward (dv and dk of a row with nothing of its own read D)"""
+    st = rnd(B, H, HD, HD, seed=1, scale=2.0)
+    st[:, :, 1] = st[:, :, 0] * (1 + 2.0 ** -12)
+    q = torch.zeros(B, 1, H, HD, dtype=dtype)
+    q[..., 0], q[..., 1] = 1.0, -1.0
+    z, sl = torch.zeros_like(q), alibi(H)
+    out, last = ops.linear_attention_fwd(q.cuda(), z.cuda(), z.cuda(), sl.cuda(), state=st.cuda(), want_state=True)
+    dq, dk, dv, first = ops.linear_attention_bwd(z.cuda(), q.cuda(), z.cuda(), sl.cuda(), z.cuda(), d_state=st.cuda(), state=st.cuda())
+    _, dk2, _, _ = ops.linear_attention_bwd(z.cuda(), z.cuda(), q.cuda(), sl.cuda(), z.cuda(), d_state=st.transpose(2, 3).contiguous().cuda())
+    lam = torch.exp(-sl.double())[:, None]
+    want = (st[:, :, 0].double() - st[:, :, 1].double()).unsqueeze(1)
+    size = (st[:, :, 0].double().abs() + st[:, :, 1].double().abs()).unsqueeze(1)
+    c = 8 * 2.0 ** -24
+    check(out, lam * want * HD ** -0.5, lam * size * HD ** -0.5, c, "out")
+    check(dv, want, size, c, "dv")
+    check(dk2, want, size, c, "dk")
+    assert not dq.any()
+    check(last, st.double() * lam.unsqueeze(-1), st.double().abs() * lam.unsqueeze(-1), c, "last")
+    check(first, st.double() * lam.unsqueeze(-1), st.double().abs() * lam.unsqueeze(-1), c, "first")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,HD,B", [(4, 32, 2), (2, 64, 2), (2, 128, 2), (16, 64, 64)])
+def test_the_values_that_a_state_sums_keep_32_bits(ops, dtype, H, HD, B):
+    """two rows whose keys are 1 and -1 and whose values are equal, a step of exp(-2^-12) apart, read a block later.  Two
+    powers to an ulp (4 half steps), a product of powers and one with the value for each of two terms (4), the parts' products added (6), two
+    more behind them: 16 roundings.  In the backward pass the same through dv and dk, without a gradient of the last state"""
+    S, sl = 70, torch.full((H,), 2.0 ** -12)
+    x = rnd(B, 1, H, HD, seed=1, dtype=dtype)
+    one = torch.zeros(B, S, H, HD, dtype=dtype)
+    e = lambda r, w: one.clone().index_fill_(1, torch.tensor(r), 1.0) * torch.tensor(w, dtype=dtype)       # noqa: E731
+    unit = torch.zeros(HD, dtype=dtype)
+    unit[3] = 1.0
+    # forward: keys e_3, -e_3 at rows 4 and 5, q = e_3 at row 69
+    k = (e([4], 1.0) - e([5], 1.0)) * unit
+    q = e([69], 1.0) * unit
+    v = (e([4], 1.0) + e([5], 1.0)) * x
+    dev = lambda *t: [y.cuda() for y in t]                    # noqa: E731
+    out, _ = ops.linear_attention_fwd(*dev(q, k, v, sl), scale=1.0)
+    w = torch.exp(-(2.0 ** -12) * torch.tensor([65.0, 64.0], dtype=torch.float64))
+    c = 16 * 2.0 ** -24
+    check(out[:, 69:], x.double() * (w[0] - w[1]), x.double().abs() * w.sum(), c, "out")
+    # backward: q e_3, -e_3 at rows 65 and 64 with gradients x; row 0 has k = e_3 (dv) or v = anything (dk)
+    q2, do = (e([65], 1.0) - e([64], 1.0)) * unit, (e([64], 1.0) + e([65], 1.0)) * x
+    _, _, dv, _ = ops.linear_attention_bwd(*dev(q2, e([0], 1.0) * unit, one, sl, do), scale=1.0)
+    w = torch.exp(-(2.0 ** -12) * torch.tensor([65.0, 64.0], dtype=torch.float64))
+    check(dv[:, :1], x.double() * (w[0] - w[1]), x.double().abs() * w.sum(), c, "dv")
+    # dk_0 = sum_t w_t (v_0 . do_t) q_t: do e_3, -e_3 with q = x
+    _, dk, _, _ = ops.linear_attention_bwd(*dev(do, one, e([0], 1.0) * unit, sl, q2), scale=1.0)
+    check(dk[:, :1], x.double() * (w[0] - w[1]), x.double().abs() * w.sum(), c, "dk")
+
+
+@gpu
+@pytest.mark.parametrize("B,S,H,HK,HD", [(1, 33, 4, 2, 64), (2, 140, 4, 4, 64), (1, 257, 2, 1, 128), (1, 200, 4, 4, 32)])
+def test_states_of_bf16_calls_are_fp32_results(ops, B, S, H, HK, HD):
+    """the state and its gradient within the bound of fp32 calls"""
+    q, k, v, do, st, ds = lin_case(B, S, H, HK, HD, torch.bfloat16, seed=41)
+    sl = alibi(H)
+    d = [t.cuda() for t in (q, k, v, do, st, ds)]
+    _, last = ops.linear_attention_fwd(d[0], d[1], d[2], sl.cuda(), state=d[4], want_state=True)
+    first = ops.linear_attention_bwd(d[0], d[1], d[2], sl.cuda(), d[3], state=d[4], d_state=d[5])[3]
+    for b in range(B):
+        t = [x[b].double() for x in (q, k, v)] + [sl, HD ** -0.5] + [x[b].double() for x in (st, do, ds)]
+        want, size = ref_linear(*t), ref_linear(*(x.abs() if torch.is_tensor(x) and x is not sl else x for x in t))
+        check(last[b], want[1], size[1], c_of(torch.float32, S, HD), "last")
+        check(first[b], want[5], size[5], c_of(torch.float32, S, HD), "first")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S,H,HK,HD", [(2300, 2, 1, 64), (4400, 1, 1, 128), (2300, 2, 2, 64)])
+def test_backward_through_the_scan(ops, dtype, S, H, HK, HD):
+    """more than 16 segments (of 2 HD rows): every segment starts from the scanned states, dk from the transposes of dv's"""
+    q, k, v, do, st, ds = lin_case(1, S, H, HK, HD, dtype, seed=13)
+    sl, scale = torch.tensor([0.001, 0.02])[:H], HD ** -0.5
+    d = [t.cuda() for t in (q, k, v, do, st, ds)]
+    got = (*ops.linear_attention_fwd(d[0], d[1], d[2], sl.cuda(), state=d[4], want_state=True),
+           *ops.linear_attention_bwd(d[0], d[1], d[2], sl.cuda(), d[3], state=d[4], d_state=d[5]))
+    t = [x[0].double() for x in (q, k, v)] + [sl, scale] + [x[0].double() for x in (st, do, ds)]
+    want, size = ref_linear(*t), ref_linear(*(x.abs() if torch.is_tensor(x) and x is not sl else x for x in t))
+    c = c_of(dtype, S, HD)
+    for g, w, m, name in zip(got, want, size, ("out", "last", "dq", "dk", "dv", "first")):
+        check(g[0], w, m, c, name)
