@@ -172,6 +172,12 @@ __device__ __forceinline__ int lin_channel(int t, int g, int i) { return 32 * (t
 __device__ __forceinline__ void lin_dma(const char* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
+// the lane, read again where it is needed: paths that are rarely taken keep nothing in registers for it
+__device__ __forceinline__ int lin_lane() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
 template <int N> __device__ __forceinline__ void lin_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 template <int IN> __device__ __forceinline__ float lin_value(const lb8 (&f)[IN], int i) {       // the element that the parts stand for
   float x = (float)f[0][i];
@@ -300,7 +306,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
   const bool o32 = r.o32;
   lin_raw pq[NU], pk[NU], pv[NU];                                // the next chunk's tiles, in flight during this one's math
   unsigned aq[NU], ak[NU], av[NU], ao[NU];
-  auto offsets = [&](unsigned (&off)[NU], long long stride, unsigned head, int c, bool in) __attribute__((always_inline)) {
+  auto offsets = [&](unsigned (&off)[NU], long long stride, unsigned head, int c, bool in, int tid) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int at = tid + u * THREADS, i = at / CPR < c ? at / CPR : c - 1;
@@ -308,15 +314,15 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
       off[u] = (unsigned)(rev ? c - 1 - i : i) * (unsigned)stride + (HEADS == 1 ? 0 : piece / CPH * head) + piece % CPH * 16;
     }
   };
-  auto offsets_in = [&](int c) __attribute__((always_inline)) {
-    if constexpr (!STATE) offsets(aq, qs, (unsigned)r.q.h, c, true);
-    offsets(ak, ks, (unsigned)r.k.h, c, true);
-    offsets(av, vs, (unsigned)r.v.h, c, true);
+  auto offsets_in = [&](int c, int tid) __attribute__((always_inline)) {
+    if constexpr (!STATE) offsets(aq, qs, (unsigned)r.q.h, c, true, tid);
+    offsets(ak, ks, (unsigned)r.k.h, c, true, tid);
+    offsets(av, vs, (unsigned)r.v.h, c, true, tid);
   };
   const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)sm + wave * 1024;
   auto fetch = [&](int c, int stage) __attribute__((always_inline)) {
     if (c < C) {
-      offsets_in(c);
+      offsets_in(c, wave * 64 + lin_lane());
       if (rev) { bq += (C - c) * qs; bk += (C - c) * ks; bv += (C - c) * vs; }
     }
 #pragma unroll
@@ -349,8 +355,8 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
     for (int k = 0; k < LIN_MID; ++k)
       if (wi == 0) *(lin_half*)(sP + k * PPART + fr * PP + 16 * g + 8) = (lin_half){0u, 0u};
   }
-  offsets_in(C);
-  if constexpr (!STATE) offsets(ao, os, (unsigned)r.o.h, C, false);
+  offsets_in(C, tid);
+  if constexpr (!STATE) offsets(ao, os, (unsigned)r.o.h, C, false, tid);
   auto rows_at = [&](int t) __attribute__((always_inline)) { return upto - t < C ? upto - t : C; };
   if (from < upto) fetch(rows_at(from), 0);
 
@@ -501,6 +507,31 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
     }
     if constexpr (!STATE || !DMA) __syncthreads();
     if constexpr (!STATE) {
+      // A value that is not finite would meet the zero weights of the rows in front of it, and 0 * inf is NaN: such values leave the product, and
+      // the rows that they reach are NaN.  (minus one's matrix, mostly zeros, shows them: a channel with one is not finite in any column.)
+      const f32x4 probe = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[0], minus.of[0], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bad |= !__builtin_isfinite(probe[i]);
+      if (__builtin_expect(__any(bad), 0)) {
+        const int lane = lin_lane(), fr = lane & 15, g = lane >> 4;
+        int row = C;                                             // first row of channel n0 + fr that is not finite
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+          const bool ok = __builtin_isfinite((float)vf[0][i]);
+          row = ok ? row : 16 * (i >> 2) + 4 * g + (i & 3);
+#pragma unroll
+          for (int k = 0; k < L::IN; ++k) vf[k][i] = ok ? vf[k][i] : (__bf16)0.f;
+        }
+        row = min(row, __shfl_xor(row, 16, 64));
+        row = min(row, __shfl_xor(row, 32, 64));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                            // (of the channel and the two rows that an accumulator holds)
+          const int r0 = __shfl(row, 4 * g + i, 64);
+          if (fr >= r0) acc[0][i] = __builtin_nanf("");
+          if (16 + fr >= r0) acc[1][i] = __builtin_nanf("");
+        }
+      }
 #pragma unroll
       for (int ti = 0; ti < 2; ++ti) {
         lb8 p[LIN_MID];
@@ -525,7 +556,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
       // operands need: 2 to 5 % on every long case.
       if (!o32) {
         if (END && c < C) {
-          offsets(ao, os, (unsigned)r.o.h, c, false);
+          offsets(ao, os, (unsigned)r.o.h, c, false, wave * 64 + lin_lane());
           if (rev) bo += (C - c) * os;
         }
 #pragma unroll

@@ -215,8 +215,8 @@ size_t a2v_qk_norm_rope_workspace(int N, int S, int H, int HK, int HD);
  * outside every sequence are left alone, or set to 0 with zero_outside.  Offsets outside [0, S] are clamped.
  * ws: a2v_linear_attention_workspace() bytes (0 where the axis is not split), 16-byte aligned; used by this call only.
  * dtype A2V_F32 or A2V_BF16; liba2v_hip_f16.so refuses its 16-bit type (A2V_ERR_UNSUPPORTED: a state does not fit half's range).
- * A non-finite value reaches the rows of its own 32-row block and those behind it (gradients of k and v: in
- * front of it), never another sequence.
+ * A value that is not finite reaches what the formula says: its own row and those behind it (gradients of k and v: in front of it).  What
+ * would be infinite may be NaN.
  * Limits, else A2V_ERR_ARG: fewer than 2^30 rows, rows less than 64 MiB apart, H / HK <= 1024, H HD HD < 2^28, fewer
  * than 2^31 / 3 / H segments. */
 int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, const float* slopes,

@@ -128,3 +128,76 @@ def test_backward_through_the_scan(ops, dtype, S, H, HK, HD):
     c = c_of(dtype, S, HD)
     for g, w, m, name in zip(got, want, size, ("out", "last", "dq", "dk", "dv", "first")):
         check(g[0], w, m, c, name)
+
+
+# ------------------------------------------------------------------------------------------------ values that are not finite
+# which elements of which result a value that is not finite reaches: (its own row and those behind or in front of it, or its own alone;
+# its own channel or all)
+REACH = {"q": dict(out=("own", "all"), dk=("front", "channel"), dv=("front", "all")),
+         "k": dict(out=("behind", "all"), dq=("behind", "channel"), dv=("own", "all")),
+         "v": dict(out=("behind", "channel"), dq=("behind", "all"), dk=("own", "all")),
+         "d_out": dict(dq=("own", "all"), dk=("front", "all"), dv=("front", "channel"))}
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,S,H,HD,row", [(2, 75, 2, 32, 40), (2, 75, 2, 64, 74), (1, 70, 3, 128, 13), (1, 45, 2, 64, 44), (64, 70, 16, 64, 37), (64, 70, 32, 32, 33), (1, 700, 2, 64, 300),
+                                          (1, 33, 2, 64, 0), (1, 1300, 1, 32, 1295)])
+def test_values_that_are_not_finite_reach_what_the_formula_says(ops, B, S, H, HD, row, dtype):
+    """one NaN or infinity in q, k, v or d_out: everything that it does not reach has the bits that it has beside a finite value, also in the
+    same block of rows and beside copies of a last row; everything that it reaches is not finite"""
+    q, k, v, do, _, _ = lin_case(B, S, H, H, HD, dtype, seed=51, state=False)
+    dev = {n: t.cuda() for n, t in (("q", q), ("k", k), ("v", v), ("d_out", do))}
+    sl, b, h, ch = (alibi(H) * 0.05).cuda(), B - 1, H - 1, HD - 3
+
+    def run(d):
+        o = ops.linear_attention_fwd(d["q"], d["k"], d["v"], sl, want_state=True)
+        g = ops.linear_attention_bwd(d["q"], d["k"], d["v"], sl, d["d_out"])
+        return dict(out=o[0], last=o[1], dq=g[0], dk=g[1], dv=g[2])
+    clean = run(dev)
+    for name, bad in (("q", "nan"), ("k", "inf"), ("v", "nan"), ("v", "inf"), ("v", "-inf"), ("k", "nan"), ("d_out", "-inf"), ("q", "inf"), ("d_out", "nan")):
+        x = dev[name].clone()
+        x[b, row, h, ch] = float(bad)
+        got = run({**dev, name: x})
+        for res in ("out", "dq", "dk", "dv"):
+            hit = torch.zeros_like(clean[res], dtype=torch.bool)
+            if res in REACH[name]:
+                where, what = REACH[name][res]
+                rows = slice(row, row + 1) if where == "own" else slice(row, None) if where == "behind" else slice(0, row + 1)
+                hit[b, rows, h, ch if what == "channel" else slice(None)] = True
+            assert torch.equal(got[res][~hit], clean[res][~hit]), (name, bad, res)
+            assert not torch.isfinite(got[res][hit]).any(), (name, bad, res)
+        hit = torch.zeros_like(clean["last"], dtype=torch.bool)
+        if name == "k":
+            hit[b, h, ch] = True
+        if name == "v":
+            hit[b, h, :, ch] = True
+        assert torch.equal(got["last"][~hit], clean["last"][~hit]) and not torch.isfinite(got["last"][hit]).any(), (name, bad)
+
+
+@gpu
+def test_values_that_are_not_finite_in_packed_sequences(ops):
+    """a NaN in the last row of a sequence, which the rows that its last block lacks are copies of, and in the first of the next one: the rows
+    of the one in front and behind, and the other heads' share of a shared head's gradient, stay as they are"""
+    T, H, HK, HD = 190, 4, 2, 64
+    q, k, v, do = (rnd(1, T, h, HD, seed=i, dtype=torch.bfloat16).cuda() for i, h in enumerate((H, HK, HK, H)))
+    cu, sl = torch.tensor([0, 45, 112, 190], dtype=torch.int32, device="cuda"), (alibi(H) * 0.1).cuda()
+    out = ops.linear_attention_fwd(q, k, v, sl, cu_seqlens=cu)[0]
+    grads = ops.linear_attention_bwd(q, k, v, sl, do, cu_seqlens=cu)[:3]
+    x, d = v.clone(), do.clone()
+    x[0, 111, 1, 7], x[0, 112, 0, 5] = float("inf"), float("nan")
+    d[0, 44, 3, 9], d[0, 45, 0, 2] = float("nan"), float("inf")
+    got = ops.linear_attention_fwd(q, k, x, sl, cu_seqlens=cu)[0]
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, 111:112, 2:, 7] = hit[0, 112:, :2, 5] = True
+    assert torch.equal(got[~hit], out[~hit]) and not torch.isfinite(got[hit]).any()
+    dq, dk, dv = ops.linear_attention_bwd(q, k, v, sl, d, cu_seqlens=cu)[:3]
+    hit = torch.zeros_like(dq, dtype=torch.bool)
+    hit[0, 44, 3] = hit[0, 45, 0] = True
+    assert torch.equal(dq[~hit], grads[0][~hit]) and not torch.isfinite(dq[hit]).any()
+    hit = torch.zeros_like(dv, dtype=torch.bool)
+    hit[0, :45, 1, 9] = hit[0, 45, 0, 2] = True
+    assert torch.equal(dv[~hit], grads[2][~hit]) and not torch.isfinite(dv[hit]).any()
+    hit = torch.zeros_like(dk, dtype=torch.bool)
+    hit[0, :45, 1] = hit[0, 45, 0] = True
+    assert torch.equal(dk[~hit], grads[1][~hit]) and not torch.isfinite(dk[hit]).any()
