@@ -48,7 +48,7 @@ struct LinRole {
   float s_inter, s_state;                                        // factors of Y^T q and of k v^T (their product is the scale)
   const float* first;                                            // (B, H, HD, HD) state before the first row, or null
   float* last;                                                   // (B, H, HD, HD) state behind the last row, or null
-  float* ws;                                                     // segment states, slots x H x HD x HD
+  float* ws;                                                     // states of all segments but the last ones, each H x HD x HD
 };
 struct LinArgs {
   LinRole r[3];
@@ -191,7 +191,9 @@ __device__ __forceinline__ void lin_store4(__bf16* p, const f32x4& v) { *(lb4*)p
 // slot -> (sequence, segment).  Sequences start wherever cu says, so sequence b gets the slots floor(start / seg) + b ...: that many are
 // always enough (ceil(len / seg) <= floor((start + len) / seg) - floor(start / seg) + 1), none is shared, and their number is known to
 // the host without reading cu.  Offsets are clamped to [0, T]: a wrong cu gives wrong rows, never an access outside the tensors.
-struct LinSeq { int b, p, np, begin, len; };                     // begin: first row, len: rows, np: segments
+// States are kept without the b: a sequence leaves one for each segment but its last, which are fewer than the multiples of seg that it
+// reaches, so floor(start / seg) + p is not shared either, and S / seg of them are enough however many sequences there are.
+struct LinSeq { int b, p, np, begin, len, kept; };               // begin: first row, len: rows, np: segments, kept: the first one's state
 __device__ __forceinline__ int lin_cu(const LinArgs& a, int b) { const int c = a.cu[b]; return c < 0 ? 0 : (c > a.T ? a.T : c); }
 __device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) {
   if (!a.cu) {
@@ -200,6 +202,7 @@ __device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) 
     s.p = slot - s.b * a.np;
     s.begin = 0;
     s.len = a.S;
+    s.kept = s.b * (a.np - 1);
     return true;
   }
   int lo = -1;                                                   // the last b in [0, B) whose first slot is <= slot: the slots ascend, so count
@@ -211,7 +214,8 @@ __device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) 
   const int end = lin_cu(a, lo + 1);
   s.len = end > s.begin ? end - s.begin : 0;
   s.np = s.len > a.seg ? (s.len + a.seg - 1) / a.seg : 1;
-  s.p = slot - (s.begin / a.seg + lo);
+  s.kept = s.begin / a.seg;
+  s.p = slot - (s.kept + lo);
   return s.p >= 0 && s.p < s.np;
 }
 __device__ __forceinline__ float lin_log2(const float* slopes, int h) {
@@ -384,7 +388,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (p0 - u <= stop) break;
-        const float* const w = r.ws + ((long long)(s.np > LIN_INLINE ? slot : slot - s.p + p0 - u - 1) * a.H + h) * HD * HD;
+        const float* const w = r.ws + ((long long)(s.kept + p0 - u - 1) * a.H + h) * HD * HD;
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
           if (!r.ws_t) x[u][t] = *(const f32x4*)(w + ((wi * ND + t) * 64 + lane) * 4);
@@ -575,7 +579,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
   }
   if (t0 < upto) chunk(std::true_type{}, t0, upto - t0, stage);
   if constexpr (STATE) {
-    f32x4* const w = (f32x4*)(r.ws + ((long long)slot * a.H + h) * HD * HD) + wi * ND * 64 + lane;
+    f32x4* const w = (f32x4*)(r.ws + ((long long)(s.kept + s.p) * a.H + h) * HD * HD) + wi * ND * 64 + lane;
 #pragma unroll
     for (int t = 0; t < ND; ++t) w[t * 64] = S[t];
   } else if (ends && r.last) {
@@ -587,7 +591,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
   }
 }
 
-// ws[slot] := the state in front of segment p from the segments before it: carried through the sequence's slots in order, one thread to an
+// The state of segment p := the state in front of segment p + 1: carried through the sequence's segments in order, one thread to an
 // element (any order of them: the waves' register image), eight loads in flight.  The part of `first` is added by the kernel that starts
 // from it.  LIN_SCANS groups of workgroups take the sequences in turn, so that the launch does not grow with their number.  (A packed batch of
 // short sequences, which have nothing to scan, pays the launch, 4.6 us: their lengths are on the device.)
@@ -601,7 +605,7 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
     const int begin = a.cu ? lin_cu(a, b) : 0, len = a.cu ? lin_cu(a, b + 1) - begin : a.S;
     const int np = len > a.seg ? (len + a.seg - 1) / a.seg : 1;
     if (np <= LIN_INLINE) continue;
-    float* const w = a.r[blockIdx.y].ws + (long long)(a.cu ? begin / a.seg + b : b * np) * step + i;
+    float* const w = a.r[blockIdx.y].ws + (long long)(a.cu ? begin / a.seg : b * (np - 1)) * step + i;
     float carry = 0.f;
     int p = 0;
     for (; p + 8 < np; p += 8) {                                 // (the last segment has no state of its own)
@@ -609,10 +613,9 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) x[u] = w[(p + u) * step];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) { w[(p + u) * step] = carry; carry = carry * f + x[u]; }
+      for (int u = 0; u < 8; ++u) w[(p + u) * step] = carry = carry * f + x[u];
     }
-    for (; p < np - 1; ++p) { const float x = w[p * step]; w[p * step] = carry; carry = carry * f + x; }
-    w[p * step] = carry;
+    for (; p < np - 1; ++p) w[p * step] = carry = carry * f + w[p * step];
   }
 }
 
@@ -728,7 +731,8 @@ static bool lin_plan(int dtype, int B, int S, int H, int HD, bool packed, LinPla
   if ((slots + 16) * H * 3 >= (1LL << 31) || (long long)H * HD * HD >= (1LL << 28)) return false;      // (a launch has at most 2^32 threads in x)
   p.slots = (int)slots;
   p.split = S > p.seg;
-  p.states = p.split ? (size_t)slots * H * HD * HD * sizeof(float) : 0;
+  const long long kept = packed ? S / p.seg : slots - B;         // every segment's but the last one's of a sequence
+  p.states = p.split ? (size_t)kept * H * HD * HD * sizeof(float) : 0;
   return true;
 }
 static bool lin_shape_ok(int B, int S, int H, int HK, int HD) {

@@ -201,3 +201,64 @@ def test_values_that_are_not_finite_in_packed_sequences(ops):
     hit = torch.zeros_like(dk, dtype=torch.bool)
     hit[0, :45, 1] = hit[0, 45, 0] = True
     assert torch.equal(dk[~hit], grads[1][~hit]) and not torch.isfinite(dk[hit]).any()
+
+
+# ------------------------------------------------------------------------------------------------ many sequences in one call
+def test_workspace_of_a_packed_call_does_not_grow_with_its_sequences():
+    """states are kept for segments that another one starts from: fewer than rows / segment, whatever the number of sequences"""
+    from animal2vec_amd import _lib
+    lib = _lib.load()
+    for rows, H, HK, HD in ((400000, 16, 16, 64), (140000, 16, 16, 128), (5000, 2, 1, 32)):
+        for back in (0, 1):
+            size = lambda B: lib.a2v_linear_attention_workspace(1, back, 1, B, rows, H, HK, HD)        # noqa: E731
+            own = size(1) - (2 * rows * H * HD * 4 if back and H != HK else 0)
+            assert own <= (back + 1) * 1024 * HD * HD * 4                  # a state for each workgroup that fills the card
+            assert all(size(B) == size(1) for B in (2, 100, 10000, 1000000))
+
+
+def packed_reference(lens, q, k, v, slopes, scale, state, d_out, d_state):
+    """ref_linear for packed rows in 64 bits, all sequences side by side"""
+    T, H, D = q.shape
+    rep, B, dev = H // k.shape[1], len(lens), q.device
+    q, k, v, d_out = (t.double() for t in (q, k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1), d_out))
+    n = torch.tensor(lens, device=dev)
+    begin, end = n.cumsum(0) - n, n.cumsum(0)
+    lam = torch.exp(-slopes.double())[:, None, None]
+    st, g = state.double().clone(), d_state.double().clone()
+    out, dq, dk, dv = (torch.zeros_like(q) for _ in range(4))
+    for i in range(max(lens)):
+        b = (n > i).nonzero()[:, 0]
+        t = begin[b] + i
+        st[b] = lam * st[b] + k[t].unsqueeze(-1) * v[t].unsqueeze(-2)
+        out[t] = scale * (q[t].unsqueeze(-1) * st[b]).sum(-2)
+        dq[t] = scale * (st[b] * d_out[t].unsqueeze(-2)).sum(-1)
+        t = end[b] - 1 - i
+        d = g[b] + scale * q[t].unsqueeze(-1) * d_out[t].unsqueeze(-2)
+        dk[t] = (d * v[t].unsqueeze(-2)).sum(-1)
+        dv[t] = (k[t].unsqueeze(-1) * d).sum(-2)
+        g[b] = lam * d
+    fold = lambda x: x.reshape(T, H // rep, rep, D).sum(2)      # noqa: E731
+    return out, st, dq, fold(dk), fold(dv), g
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,HK,HD", [(2, 1, 32), (2, 2, 64)])
+def test_many_packed_sequences(ops, dtype, H, HK, HD):
+    """thousands of short and empty sequences around ones of exactly one, two, 17 and 18 segments (of 2 HD rows) and a row more or less: a
+    neighbour's states are neither taken nor overwritten, and every sequence finds its rows"""
+    seg, r = 2 * HD, torch.Generator().manual_seed(5)
+    short = lambda n: torch.randint(0, 4, (n,), generator=r).tolist()         # noqa: E731
+    lens = [0, 0, seg, seg, 2 * seg, 1, seg - 1, seg + 1, 3 * seg, 17 * seg, 18 * seg + 1] + short(1500) + [20 * seg - 7] + short(70) + [2 * seg + 5, 0, seg, 17 * seg + 1] + short(3000)
+    T, B = sum(lens), len(lens)
+    q, k, v, do = (rnd(1, T, h, HD, seed=i, dtype=dtype).cuda() for i, h in enumerate((H, HK, HK, H)))
+    st, ds = rnd(B, H, HD, HD, seed=7, scale=2.0).cuda(), rnd(B, H, HD, HD, seed=8).cuda()
+    sl = torch.tensor([0.002, 0.03], device="cuda")
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    got = (*ops.linear_attention_fwd(q, k, v, sl, state=st, want_state=True, cu_seqlens=cu),
+           *ops.linear_attention_bwd(q, k, v, sl, do, state=st, d_state=ds, cu_seqlens=cu))
+    want = packed_reference(lens, q[0], k[0], v[0], sl, HD ** -0.5, st, do[0], ds)
+    size = packed_reference(lens, q[0].abs(), k[0].abs(), v[0].abs(), sl, HD ** -0.5, st.abs(), do[0].abs(), ds.abs())
+    c = c_of(dtype, max(lens), HD)
+    for g, w, m, name in zip(got, want, size, ("out", "last", "dq", "dk", "dv", "first")):
+        check(g[0] if name not in ("last", "first") else g, w.cpu(), m.cpu(), c, name)
