@@ -195,6 +195,18 @@ __device__ __forceinline__ void lin_store4(__bf16* p, const f32x4& v) { *(lb4*)p
 // reaches, so floor(start / seg) + p is not shared either, and S / seg of them are enough however many sequences there are.
 struct LinSeq { int b, p, np, begin, len, kept; };               // begin: first row, len: rows, np: segments, kept: the first one's state
 __device__ __forceinline__ int lin_cu(const LinArgs& a, int b) { const int c = a.cu[b]; return c < 0 ? 0 : (c > a.T ? a.T : c); }
+// the last b in [0, n) for which `is` holds, 0 if it never does: one look of the wave's 64 lanes for up to 64 sequences, two for 4096, three for
+// 262144.  (A look at 64 sequences after the other: 10000 packed clips of 140 rows took six times as long as the same clips side by side.)
+template <typename F> __device__ __forceinline__ int lin_last(int n, F is) {
+  int lo = 0;
+  for (const int lane = threadIdx.x & 63; n > 1;) {
+    const int step = (n + 63) >> 6, count = __popcll(__ballot(lane * step < n && is(lo + lane * step)));
+    const int at = count > 0 ? (count - 1) * step : 0;
+    lo += at;
+    n = n - at < step ? n - at : step;
+  }
+  return lo;
+}
 __device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) {
   if (!a.cu) {
     s.np = a.np;
@@ -205,10 +217,7 @@ __device__ __forceinline__ bool lin_find(const LinArgs& a, int slot, LinSeq& s) 
     s.kept = s.b * (a.np - 1);
     return true;
   }
-  int lo = -1;                                                   // the last b in [0, B) whose first slot is <= slot: the slots ascend, so count
-  for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) < a.B; i += 64)       // (64 sequences a look: a binary search is six loads in a row)
-    lo += __popcll(__ballot(i < a.B && lin_cu(a, i) / a.seg + i <= slot));
-  lo = lo < 0 ? 0 : lo;
+  const int lo = lin_last(a.B, [&](int b) { return lin_cu(a, b) / a.seg + b <= slot; });       // the slots ascend with b
   s.b = lo;
   s.begin = lin_cu(a, lo);
   const int end = lin_cu(a, lo + 1);
@@ -593,30 +602,36 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
 
 // The state of segment p := the state in front of segment p + 1: carried through the sequence's segments in order, one thread to an
 // element (any order of them: the waves' register image), eight loads in flight.  The part of `first` is added by the kernel that starts
-// from it.  LIN_SCANS groups of workgroups take the sequences in turn, so that the launch does not grow with their number.  (A packed batch of
-// short sequences, which have nothing to scan, pays the launch, 4.6 us: their lengths are on the device.)
-#define LIN_SCANS 8
+// from it.  A group of workgroups takes a sequence; of packed ones each that has something to scan, which reaches a multiple of LIN_INLINE
+// segments of rows: the group of the first such row looks for the sequence around it, so there are few groups however many sequences there
+// are.  (Short ones alone pay the launch, 4.8 us with 37 as with 10000 of them: their lengths are on the device.)
 __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
-  const int per = a.H * HH / 256, b0 = blockIdx.x / per;
-  const int i = (blockIdx.x - b0 * per) * 256 + threadIdx.x, h = i / HH;       // element of (H, HD, HD); HD * HD % 256 == 0
+  const int per = a.H * HH / 256, group = blockIdx.x / per;
+  const int i = (blockIdx.x - group * per) * 256 + threadIdx.x, h = i / HH;    // element of (H, HD, HD); HD * HD % 256 == 0
+  int b = group, begin = 0, len = a.S;
+  if (a.cu) {
+    const int row = group * LIN_INLINE * a.seg;
+    b = lin_last(a.B, [&](int b) { return lin_cu(a, b) <= row; });
+    begin = lin_cu(a, b);
+    const int end = lin_cu(a, b + 1);
+    if (row < begin || row >= end || row - begin >= LIN_INLINE * a.seg) return;
+    len = end - begin;
+  }
+  const int np = len > a.seg ? (len + a.seg - 1) / a.seg : 1;
+  if (np <= LIN_INLINE) return;
   const float f = lin_pow(lin_log2(a.slopes, h), a.seg);
   const long long step = (long long)a.H * HH;
-  for (int b = b0; b < a.B; b += LIN_SCANS) {
-    const int begin = a.cu ? lin_cu(a, b) : 0, len = a.cu ? lin_cu(a, b + 1) - begin : a.S;
-    const int np = len > a.seg ? (len + a.seg - 1) / a.seg : 1;
-    if (np <= LIN_INLINE) continue;
-    float* const w = a.r[blockIdx.y].ws + (long long)(a.cu ? begin / a.seg : b * (np - 1)) * step + i;
-    float carry = 0.f;
-    int p = 0;
-    for (; p + 8 < np; p += 8) {                                 // (the last segment has no state of its own)
-      float x[8];
+  float* const w = a.r[blockIdx.y].ws + (long long)(a.cu ? begin / a.seg : b * (np - 1)) * step + i;
+  float carry = 0.f;
+  int p = 0;
+  for (; p + 8 < np; p += 8) {                                   // (the last segment has no state of its own)
+    float x[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = w[(p + u) * step];
+    for (int u = 0; u < 8; ++u) x[u] = w[(p + u) * step];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) w[(p + u) * step] = carry = carry * f + x[u];
-    }
-    for (; p < np - 1; ++p) w[p * step] = carry = carry * f + w[p * step];
+    for (int u = 0; u < 8; ++u) w[(p + u) * step] = carry = carry * f + x[u];
   }
+  for (; p < np - 1; ++p) w[p * step] = carry = carry * f + w[p * step];
 }
 
 // the gradients of a shared k / v head: the sum over its heads, of fp32 rows (T, H, HD) -> rows of HK heads
@@ -757,7 +772,10 @@ static void lin_launch_heads(const LinArgs& a, const LinPlan& p, hipStream_t str
   const dim3 block(HD * HEADS * 4);
   if (p.split) {
     hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, true>), lin_grid(a, a.roles_state, HEADS), block, 0, stream, a);
-    if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) hipLaunchKernelGGL(lin_scan_kernel, dim3((unsigned)a.H * (HD * HD / 256) * (a.B < LIN_SCANS ? a.B : LIN_SCANS), a.roles_state), dim3(256), 0, stream, a, HD * HD);
+    if ((a.S + a.seg - 1) / a.seg > LIN_INLINE) {
+      const unsigned groups = a.cu ? a.S / (LIN_INLINE * a.seg) + 1 : a.B, per = a.H * (HD * HD / 256);          // (B H < LIN_WGS / 2 where sequences are cut)
+      hipLaunchKernelGGL(lin_scan_kernel, dim3(per * groups, a.roles_state), dim3(256), 0, stream, a, HD * HD);
+    }
   }
   hipLaunchKernelGGL((lin_kernel<T, HD, HEADS, false>), lin_grid(a, a.roles, HEADS), block, 0, stream, a);
 }

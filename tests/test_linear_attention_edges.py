@@ -262,3 +262,24 @@ def test_many_packed_sequences(ops, dtype, H, HK, HD):
     c = c_of(dtype, max(lens), HD)
     for g, w, m, name in zip(got, want, size, ("out", "last", "dq", "dk", "dv", "first")):
         check(g[0] if name not in ("last", "first") else g, w.cpu(), m.cpu(), c, name)
+
+
+@gpu
+def test_sequences_are_found_among_any_number(ops):
+    """1, 2, 63 ... 70000 sequences, at the edges of what one, two and three looks of 64 lanes tell apart: sequence b's rows hold b + 1 and the
+    state behind them says so"""
+    H, HD = 1, 32
+    for B in (1, 2, 63, 64, 65, 128, 4095, 4096, 4097, 4225, 70000):
+        lens = torch.randint(0, 3, (B,), generator=torch.Generator().manual_seed(B))
+        cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).to(torch.int32).cuda() + 3
+        T = int(cu[-1]) + 200
+        of = torch.repeat_interleave(torch.arange(1, B + 1), lens).float().cuda()
+        k = torch.full((1, T, H, HD), 9.0, device="cuda")
+        v = torch.zeros(1, T, H, HD, device="cuda")
+        k[0, 3:T - 200], v[0, 3:T - 200, 0, 0] = 1.0, of
+        out, last = ops.linear_attention_fwd(k, k, v, torch.zeros(H, device="cuda"), scale=1.0, cu_seqlens=cu, want_state=True)
+        want = lens.cuda() * torch.arange(1, B + 1, device="cuda")         # (below 2^24: exact)
+        assert torch.equal(last[:, 0, :, 0], want.float()[:, None].expand(B, HD)) and not last[:, 0, :, 1:].any(), B
+        first = torch.cat([torch.ones(1, device="cuda"), (of[1:] != of[:-1]).float()]) if len(of) else of
+        assert torch.equal(out[0, 3:T - 200, 0, 0], HD * of * (2 - first)), B
+        assert not out[0, :3].any() and not out[0, T - 200:].any(), B
