@@ -36,6 +36,7 @@ typedef __attribute__((ext_vector_type(8))) __bf16 lb8;
 
 typedef __attribute__((ext_vector_type(4))) unsigned lin_raw;     // 16 bytes in flight
 typedef __attribute__((ext_vector_type(2))) unsigned lin_half;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
 
 struct LinOperand { const char* p; long long n, s, h; };        // address; bytes between sequences, rows, heads
 struct LinRole {
@@ -662,62 +663,85 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const float* dk32, const 
 // slots[n] names the state of row n.  Rows that name the same slot are successive tokens of one stream, in row order: the workgroup of
 // the first of them takes them all (the others find an earlier row and leave), so there is no race and no order left open.  A slot
 // outside [0, n_slots) leaves every state alone and gives a row of zeros (padding rows of a captured graph).
+// So a workgroup reads all slots, which grows with the square of N.  It therefore takes N / LIN_STEP_SLOTS heads of its row one after the other: fewer
+// workgroups for each row, and never so few that the card is not full (16 heads of 64 channels: 40000 rows 4.3 ms against 12.3 with one head to
+// a workgroup, 10000 1.08 against 1.45, 3.9 and 0.97 without slots; 700 rows 56 us, 66 with a limit of 128).
+#define LIN_STEP_SLOTS 512
 struct LinStep {
   const void* q; const void* k; const void* v; void* o;
   long long qn, qh, kn, kh, vn, vh, on, oh;
   const float* slopes; float* state; const int* slots;
-  int n_slots, N, H, rep;
+  int n_slots, N, H, rep, heads;                                 // heads: of a workgroup
   float scale;
 };
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void lin_step_kernel(LinStep a) {
   constexpr int LPR = HD / 4, RPP = 256 / LPR, NP = HD / RPP;    // lanes of a row, rows of a pass, passes
   __shared__ f32x4 part[4 * LPR];
-  const int n = blockIdx.x / a.H, h = blockIdx.x - n * a.H, tid = threadIdx.x, hk = h / a.rep;
+  const int groups = (a.H + a.heads - 1) / a.heads, n = blockIdx.x / groups, tid = threadIdx.x;
+  const int h0 = (blockIdx.x - n * groups) * a.heads, h1 = h0 + a.heads < a.H ? h0 + a.heads : a.H;
   const int c = (tid % LPR) * 4, r0 = tid / LPR;
   const int slot = a.slots ? a.slots[n] : n;
-  T* const out = (T*)a.o + h * a.oh;
+  T* const out = (T*)a.o;
   if (slot < 0 || slot >= a.n_slots) {
-    if (tid < LPR) Vec4<T>::store(out + n * a.on + c, (f32x4){0.f, 0.f, 0.f, 0.f});
+    for (int h = h0; h < h1; ++h)
+      if (tid < LPR) Vec4<T>::store(out + n * a.on + h * a.oh + c, (f32x4){0.f, 0.f, 0.f, 0.f});
     return;
   }
-  float* const st = a.state + ((long long)slot * a.H + h) * HD * HD;
+  float* const st = a.state + (long long)slot * a.H * HD * HD + r0 * HD + c;
   f32x4 S[NP];
 #pragma unroll
-  for (int p = 0; p < NP; ++p) S[p] = *(const f32x4*)(st + (r0 + p * RPP) * HD + c);
+  for (int p = 0; p < NP; ++p) S[p] = *(const f32x4*)(st + ((long long)h0 * HD + p * RPP) * HD);
   bool more = false;
   if (a.slots) {
     bool before = false;
-    for (int m = tid; m < a.N; m += 256)
-      if (a.slots[m] == slot) { before |= m < n; more |= m > n; }
+    auto look = [&](int m, int other) __attribute__((always_inline)) { before |= m < n && other == slot; more |= m > n && other == slot; };
+    const int lead = (int)(-(uintptr_t)a.slots >> 2 & 3), quads = a.N > lead ? (a.N - lead) >> 2 : 0;        // 16 bytes a lane between the ends
+    for (int i = tid; i < quads; i += 256) {
+      const int m = lead + 4 * i;
+      const i32x4 x = *(const i32x4*)(a.slots + m);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) look(m + u, x[u]);
+    }
+    if (tid < 8) {
+      const int m = tid < 4 ? tid : lead + 4 * quads + tid - 4;
+      if (tid < 4 ? m < lead && m < a.N : m < a.N) look(m, a.slots[m]);
+    }
     if (__syncthreads_or(before)) return;
     more = __syncthreads_or(more);
   }
-  const float l = lin_pow(lin_log2(a.slopes, h), 1);
-  for (int m = n; m < a.N; ++m) {
-    if (m > n && a.slots[m] != slot) continue;
-    const T* const q = (const T*)a.q + m * a.qn + h * a.qh;
-    const T* const k = (const T*)a.k + m * a.kn + hk * a.kh;
-    const f32x4 v = Vec4<T>::load((const T*)a.v + m * a.vn + hk * a.vh + c);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int h = h0; h < h1; ++h) {
+    const int hk = h / a.rep;
+    const float l = lin_pow(lin_log2(a.slopes, h), 1);
+    for (int m = n; m < a.N; ++m) {
+      if (m > n && a.slots[m] != slot) continue;
+      const T* const q = (const T*)a.q + m * a.qn + h * a.qh;
+      const T* const k = (const T*)a.k + m * a.kn + hk * a.kh;
+      const f32x4 v = Vec4<T>::load((const T*)a.v + m * a.vn + hk * a.vh + c);
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int d = r0 + p * RPP;
-      S[p] = S[p] * l + v * ldf(k + d);
-      o += S[p] * ldf(q + d);
+      for (int p = 0; p < NP; ++p) {
+        const int d = r0 + p * RPP;
+        S[p] = S[p] * l + v * ldf(k + d);
+        o += S[p] * ldf(q + d);
+      }
+#pragma unroll
+      for (int x = LPR; x < 64; x <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+      if ((tid & 63) < LPR) part[(tid >> 6) * LPR + (tid & 63)] = o;
+      __syncthreads();
+      if (tid < LPR) Vec4<T>::store(out + m * a.on + h * a.oh + c, (part[tid] + part[LPR + tid] + part[2 * LPR + tid] + part[3 * LPR + tid]) * a.scale);
+      if (!more && h + 1 == h1) break;
+      __syncthreads();
+      if (!more) break;
     }
 #pragma unroll
-    for (int x = LPR; x < 64; x <<= 1)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
-    if ((tid & 63) < LPR) part[(tid >> 6) * LPR + (tid & 63)] = o;
-    __syncthreads();
-    if (tid < LPR) Vec4<T>::store(out + m * a.on + c, (part[tid] + part[LPR + tid] + part[2 * LPR + tid] + part[3 * LPR + tid]) * a.scale);
-    if (!more) break;
-    __syncthreads();
+    for (int p = 0; p < NP; ++p) {
+      *(f32x4*)(st + ((long long)h * HD + p * RPP) * HD) = S[p];
+      if (h + 1 < h1) S[p] = *(const f32x4*)(st + ((long long)(h + 1) * HD + p * RPP) * HD);
+    }
   }
-#pragma unroll
-  for (int p = 0; p < NP; ++p) *(f32x4*)(st + (r0 + p * RPP) * HD + c) = S[p];
 }
 
 // ------------------------------------------------------------------------------------------------------------------ host side
@@ -910,7 +934,7 @@ extern "C" int a2v_linear_attention_step(int dtype, const void* q, const void* k
                                          const float* slopes, float* state, const int* slots, int n_slots, int N, int H, int HK, int HD, float scale,
                                          hipStream_t stream) {
   if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
-  if (!strides || !slopes || !state || ((uintptr_t)state & 15) || N < 0 || H <= 0 || HK <= 0 || H % HK || (HD != 32 && HD != 64 && HD != 128) ||
+  if (!strides || !slopes || !state || ((uintptr_t)state & 15) || ((uintptr_t)slots & 3) || N < 0 || H <= 0 || HK <= 0 || H % HK || (HD != 32 && HD != 64 && HD != 128) ||
       n_slots < (slots ? 0 : N) || (long long)N * H >= (1LL << 24))              // (2^32 threads)
     return A2V_ERR_ARG;
   if (N == 0) return A2V_OK;
@@ -918,9 +942,10 @@ extern "C" int a2v_linear_attention_step(int dtype, const void* q, const void* k
   const void* const t[4] = {q, k, v, out};
   for (int i = 0; i < 4; ++i)
     if (!t[i] || ((uintptr_t)t[i] & (4 * es - 1)) || strides[2 * i] % 4 || strides[2 * i + 1] % 4) return A2V_ERR_ARG;
+  const int heads = !slots || N < LIN_STEP_SLOTS ? 1 : N / LIN_STEP_SLOTS < H ? N / LIN_STEP_SLOTS : H;
   const LinStep a{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
-                  slopes, state, slots, n_slots, N, H, H / HK, scale};
-  const dim3 grid((unsigned)(N * H)), block(256);
+                  slopes, state, slots, n_slots, N, H, H / HK, heads, scale};
+  const dim3 grid((unsigned)(N * ((H + heads - 1) / heads))), block(256);
 #define LIN_STEP(T_, HD_) hipLaunchKernelGGL((lin_step_kernel<T_, HD_>), grid, block, 0, stream, a)
   if (dtype == A2V_F32) { if (HD == 32) LIN_STEP(float, 32); else if (HD == 64) LIN_STEP(float, 64); else LIN_STEP(float, 128); }
   else { if (HD == 32) LIN_STEP(bf16, 32); else if (HD == 64) LIN_STEP(bf16, 64); else LIN_STEP(bf16, 128); }

@@ -283,3 +283,32 @@ def test_sequences_are_found_among_any_number(ops):
         first = torch.cat([torch.ones(1, device="cuda"), (of[1:] != of[:-1]).float()]) if len(of) else of
         assert torch.equal(out[0, 3:T - 200, 0, 0], HD * of * (2 - first)), B
         assert not out[0, :3].any() and not out[0, T - 200:].any(), B
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,H,HK,HD,pool,shift", [(511, 3, 1, 32, 200, 1), (512, 2, 2, 64, 600, 0), (1100, 4, 2, 32, 300, 2), (1700, 4, 4, 64, 1500, 3), (3001, 4, 1, 32, 3500, 1), (5, 2, 1, 32, 3, 3)])
+def test_step_of_many_rows(ops, N, H, HK, HD, pool, shift, dtype):
+    """several heads to a workgroup (a number that need not divide them), slots that start anywhere, named once, often, or outside the pool"""
+    r = torch.Generator().manual_seed(N)
+    slots = torch.randint(-3, pool + 3, (N + shift,), generator=r, dtype=torch.int32)
+    qkv = rnd(N, H + 2 * HK, HD, seed=1, dtype=dtype)
+    state, sl, scale = rnd(pool, H, HD, HD, seed=2), alibi(H), HD ** -0.5
+    sd, x = state.cuda(), qkv.cuda()
+    out = ops.linear_attention_step(x[:, :H], x[:, H:H + HK], x[:, H + HK:], sl.cuda(), sd, slots=slots.cuda()[shift:])
+    sel = slots[shift:].tolist()
+    lam = torch.exp(-sl.double())[:, None, None]
+    want, size = state.double(), state.double().abs()
+    o, m = torch.zeros(N, H, HD, dtype=torch.float64), torch.zeros(N, H, HD, dtype=torch.float64)
+    count = [0] * pool
+    for n, s in enumerate(sel):
+        if 0 <= s < pool:
+            q, k, v = (t.double() for t in (qkv[n, :H], qkv[n, H:H + HK].repeat_interleave(H // HK, 0), qkv[n, H + HK:].repeat_interleave(H // HK, 0)))
+            kv = k.unsqueeze(-1) * v.unsqueeze(-2)
+            want[s], size[s] = lam * want[s] + kv, lam * size[s] + kv.abs()
+            o[n], m[n] = scale * (q.unsqueeze(-1) * want[s]).sum(-2), scale * (q.abs().unsqueeze(-1) * size[s]).sum(-2)
+            count[s] += 1
+    c = (HD + 16 + 4 * max(count)) * 2.0 ** -24
+    check(out, o, m, c, "out")
+    check(sd, want, size, c, "states")
+    assert not out[[n for n, s in enumerate(sel) if not 0 <= s < pool]].any()
