@@ -715,8 +715,8 @@ def _strides(*ts):
 
 
 def _like(t):
-    """a contiguous tensor of t's layout, at capacity inside an engine step (set_row_cap)"""
-    return torch.empty_like(t, memory_format=torch.contiguous_format) if _ROWCAP is None else _E(*t.shape, dtype=t.dtype, device=t.device)
+    """a contiguous tensor of t's shape and type"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _qk_norm_rope_checks(what, q, k, q_weight, k_weight, inv_freq, pos, sections):
