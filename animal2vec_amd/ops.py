@@ -658,20 +658,35 @@ def _on_gpu(t):
 
 
 def _overlap(a, b):
-    """whether two tensors of heads may share an element: exact for slots of one packed buffer (equal row strides), else by address range"""
+    """whether two tensors of heads share an element: whether the distance of their starts is a sum of strides times differences of indices
+    (said of very irregular strides without a proof)"""
     if a.numel() == 0 or b.numel() == 0:
         return False
-    es = a.element_size()
-    ext = [sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 for t in (a, b)]
-    d = (a.data_ptr() - b.data_ptr()) // es
-    if d >= ext[1] or -d >= ext[0]:
-        return False
-    rows = [s for n, s in zip(a.shape[:-2], a.stride()) if n > 1]
-    if a.shape[:-2] != b.shape[:-2] or rows != [s for n, s in zip(b.shape[:-2], b.stride()) if n > 1] or not rows or min(rows) <= 0 or any(s % min(rows) for s in rows):
-        return True
-    wide = [(t.shape[-2] - 1) * t.stride(-2) + t.shape[-1] for t in (a, b)]          # what a row of each covers, compared modulo the row pitch
-    d %= min(rows)
-    return d < wide[1] or min(rows) - d < wide[0]
+    span = {}                                                    # stride -> smallest and largest difference of the indices it goes with
+    for t, other in ((a, 0), (b, 1)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s:
+                low, high = span.get(s, (0, 0))
+                span[s] = (low - n + 1, high) if other else (low, high + n - 1)
+    terms = sorted(((s, *r) for s, r in span.items()), reverse=True)
+    low, high = [0], [0]                                         # of the sums over the terms from i on
+    for s, x, y in reversed(terms):
+        low.insert(0, low[0] + s * x)
+        high.insert(0, high[0] + s * y)
+    todo, looks = [(0, (b.data_ptr() - a.data_ptr()) // a.element_size())], 0
+    while todo:
+        i, rest = todo.pop()
+        if not low[i] <= rest <= high[i]:
+            continue
+        if i == len(terms):
+            return True                                          # (rest is 0)
+        s, x, y = terms[i]
+        first, last = max(x, -((high[i + 1] - rest) // s)), min(y, (rest - low[i + 1]) // s)
+        looks += 1 + last - first
+        if looks > 4096:
+            return True
+        todo += [(i + 1, rest - s * n) for n in range(first, last + 1)]
+    return False
 
 
 def _apart(what, outs, ins, inplace=False):

@@ -312,3 +312,70 @@ def test_step_of_many_rows(ops, N, H, HK, HD, pool, shift, dtype):
     check(out, o, m, c, "out")
     check(sd, want, size, c, "states")
     assert not out[[n for n, s in enumerate(sel) if not 0 <= s < pool]].any()
+
+
+# ------------------------------------------------------------------------------------------------ tensors that share a buffer
+def test_overlap_is_what_the_elements_say():
+    """small strided views of one buffer against their elements one by one"""
+    import itertools
+    import random
+    from animal2vec_amd import ops
+    r, buf, met = random.Random(1), torch.zeros(4000, dtype=torch.bfloat16), 0
+
+    def view():
+        dims = r.randint(2, 4)
+        return buf.as_strided([r.randint(1, 4) for _ in range(dims)], [r.choice([0, 1, 2, 3, 5, 8, 12, 16, 24, 40, 64, 96, 200]) for _ in range(dims)], r.randint(0, 600))
+
+    def elements(t):
+        return {t.storage_offset() + sum(i * s for i, s in zip(at, t.stride())) for at in itertools.product(*map(range, t.shape))}
+    for _ in range(4000):
+        a, b = view(), view()
+        share = bool(elements(a) & elements(b))
+        assert ops._overlap(a, b) == share, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        met += share
+    assert 100 < met < 3900
+
+
+PACKED = {"heads outermost": (lambda n, s, h, d: (n, s, h, 3, d), 3, (0, 1, 2, 3)), "slots outermost": (lambda n, s, h, d: (3, n, s, h, d), 0, (0, 1, 2, 3)),
+          "rows innermost": (lambda n, s, h, d: (n, 3, h, s, d), 1, (0, 2, 1, 3)), "rows of heads": (lambda n, s, h, d: (n, h, 3, s, d), 2, (0, 2, 1, 3))}
+
+
+def packed_slots(layout, N, S, H, HD, **kw):
+    shape, dim, order = PACKED[layout]
+    return [t.permute(order) for t in torch.zeros(*shape(N, S, H, HD), **kw).unbind(dim)]
+
+
+@pytest.mark.parametrize("layout", PACKED)
+def test_slots_of_any_packed_buffer_are_taken(layout):
+    """results beside each other in one buffer, whichever dimension the slots lie between, reach the device check; a slot moved onto its
+    neighbour does not"""
+    from animal2vec_amd import _lib, ops
+    N, S, H, HD = 2, 5, 4, 64
+    q, k, v = packed_slots(layout, N, S, H, HD, dtype=torch.bfloat16)
+    g = packed_slots(layout, N, S, H, HD, dtype=torch.bfloat16)
+    w, f, sl, do = torch.zeros(HD), torch.zeros(HD // 2), torch.zeros(H), torch.zeros(N, S, H, HD, dtype=torch.bfloat16)
+    for go in (lambda: ops.linear_attention_bwd(q, k, v, sl, do, dq=g[0], dk=g[1], dv=g[2]), lambda: ops.linear_attention_fwd(q, k, do, sl, out=v),
+               lambda: ops.qk_norm_rope_fwd(q, k, w, w, f, q_out=q, k_out=k)):
+        with pytest.raises(_lib.A2VError):
+            go()
+    onto = g[1].as_strided(g[1].shape, g[1].stride(), g[1].storage_offset() - HD // 2)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.linear_attention_bwd(q, k, v, sl, do, dq=g[0], dk=onto, dv=g[2])
+
+
+@gpu
+@pytest.mark.parametrize("layout", PACKED)
+def test_results_in_slots_of_any_packed_buffer(ops, layout):
+    N, S, H, HD = 2, 75, 4, 64
+    q, k, v = packed_slots(layout, N, S, H, HD, dtype=torch.bfloat16, device="cuda")
+    for i, t in enumerate((q, k, v)):
+        t.copy_(rnd(N, S, H, HD, seed=i))
+    do, sl, w, f = rnd(N, S, H, HD, seed=4, dtype=torch.bfloat16).cuda(), alibi(H).cuda(), 1 + 0.1 * rnd(HD, seed=5).cuda(), ops.rope_inv_freq((HD // 2,))
+    want = ops.linear_attention_bwd(q.contiguous(), k.contiguous(), v.contiguous(), sl, do)[:3]
+    g = packed_slots(layout, N, S, H, HD, dtype=torch.bfloat16, device="cuda")
+    for _ in range(2):
+        ops.linear_attention_bwd(q, k, v, sl, do, dq=g[0], dk=g[1], dv=g[2])
+    assert all(torch.equal(a, b) for a, b in zip(g, want))
+    want, kept = ops.qk_norm_rope_fwd(q.contiguous(), k.contiguous(), w, w, f), v.clone()
+    ops.qk_norm_rope_fwd(q, k, w, w, f, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, kept)
