@@ -48,37 +48,50 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build(force: bool = False, verbose: bool = True) -> str:
-    os.makedirs(OBJ, exist_ok=True)
+HEADERS = [os.path.join(CSRC, h) for h in ("a2v_common.h", "a2v_gemm.h", "a2v_attn_seq2.h")]
+
+
+def _made_by(target: str, cmd) -> bool:
+    """whether `target` came from this command: flags are part of what a built file depends on"""
+    try:
+        with open(target + ".cmd") as f:
+            return f.read() == " ".join(cmd)
+    except OSError:
+        return False
+
+
+def _run(target: str, deps, cmd, what: str, force: bool, verbose: bool) -> bool:
+    """runs `cmd`, which makes `target`, unless that is newer than `deps` and was made by the same command; -> whether it ran"""
+    if not force and not _stale(target, deps) and _made_by(target, cmd):
+        return False
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        raise RuntimeError(f"{what} failed:\n{r.stderr}")
+    with open(target + ".cmd", "w") as f:
+        f.write(" ".join(cmd))
+    return True
+
+
+def _objects(sources, obj_dir: str, defines, force: bool, verbose: bool):
+    """compiles what is out of date -> the objects, whether any was compiled"""
+    os.makedirs(obj_dir, exist_ok=True)
     hipcc = _hipcc()
-    hdrs = [os.path.join(CSRC, "a2v_common.h"), os.path.join(CSRC, "a2v_gemm.h"), os.path.join(CSRC, "a2v_attn_seq2.h")]
-    jobs = []
-    for s in SOURCES:
-        src, obj = os.path.join(CSRC, s), os.path.join(OBJ, s.replace(".hip", ".o"))
-        if force or _stale(obj, [src, *hdrs]):
-            jobs.append((src, obj))
+    objs = [os.path.join(obj_dir, s.replace(".hip", ".o")) for s in sources]
 
     def cc(job):
-        src, obj = job
-        cmd = [hipcc, *FLAGS, *FILE_FLAGS.get(os.path.basename(src), []), "-c", src, "-o", obj]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode:
-            raise RuntimeError(f"hipcc failed on {src}:\n{r.stderr}")
-        return obj
+        s, obj = job
+        src = os.path.join(CSRC, s)
+        return _run(obj, [src, *HEADERS], [hipcc, *FLAGS, *defines, *FILE_FLAGS.get(s, []), "-c", src, "-o", obj], f"hipcc on {src}", force, verbose)
+    with ThreadPoolExecutor(max_workers=8) as ex:
+        return objs, any(list(ex.map(cc, zip(sources, objs))))
 
-    with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(cc, jobs))
-    objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in SOURCES]
-    if force or jobs or _stale(LIB, objs):
-        cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode:
-            raise RuntimeError(f"link failed:\n{r.stderr}")
-    build_abi_client(force=force or bool(jobs), verbose=verbose)
+
+def build(force: bool = False, verbose: bool = True) -> str:
+    objs, made = _objects(SOURCES, OBJ, [], force, verbose)
+    _run(LIB, objs, [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs], "link", force or made, verbose)
+    build_abi_client(force=force or made, verbose=verbose)
     # the fp16 twin (csrc/a2v_common.h: A2V_ELT_F16): same sources, IEEE half as the 16-bit type -- the EMA teacher's forward
     build_variant("f16", ["-DA2V_ELT_F16"], verbose=verbose, force=force)
     return LIB
@@ -91,14 +104,9 @@ def build_abi_client(force: bool = False, verbose: bool = True) -> str:
     out = os.path.join(root, "tests", "abi_client", "abi_client.bin")
     if not os.path.exists(src):
         return ""
-    if force or _stale(out, [src, os.path.join(root, "include", "a2v.h"), LIB]):
-        cmd = [_hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", os.path.join(root, "include"), src, "-o", out,
-               "-L", HERE, "-la2v_hip", "-Wl,-rpath,$ORIGIN/../../animal2vec_amd"]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode:
-            raise RuntimeError(f"abi client build failed:\n{r.stderr}")
+    _run(out, [src, os.path.join(root, "include", "a2v.h"), LIB],
+         [_hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17", *NO_PACKED, "-I", os.path.join(root, "include"), src, "-o", out,
+          "-L", HERE, "-la2v_hip", "-Wl,-rpath,$ORIGIN/../../animal2vec_amd"], "abi client build", force, verbose)
     return out
 
 
@@ -106,29 +114,10 @@ def build_variant(tag: str, defines, verbose: bool = False, force: bool = False)
     """Experiment / diagnostic builds next to the product library (liba2v_hip_<tag>.so, own object directory): same sources with
     extra -D switches, e.g. build_variant("stamp", ["-DP8_STAMP"]) for tools/inkernel_clock.py.  Selected at run time with
     A2V_LIB_PATH; never loaded by default, never built by build()."""
-    obj_dir = os.path.join(CSRC, "build_" + tag)
-    os.makedirs(obj_dir, exist_ok=True)
     lib = os.path.join(HERE, f"liba2v_hip_{tag}.so")
-    hipcc = _hipcc()
-    hdrs = [os.path.join(CSRC, "a2v_common.h"), os.path.join(CSRC, "a2v_gemm.h"), os.path.join(CSRC, "a2v_attn_seq2.h")]
-
-    def cc(s):
-        src, obj = os.path.join(CSRC, s), os.path.join(obj_dir, s.replace(".hip", ".o"))
-        if force or _stale(obj, [src, *hdrs]):
-            cmd = [hipcc, *FLAGS, *defines, *FILE_FLAGS.get(s, []), "-c", src, "-o", obj]
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            r = subprocess.run(cmd, capture_output=True, text=True)
-            if r.returncode:
-                raise RuntimeError(f"hipcc failed on {src}:\n{r.stderr}")
-        return obj
-
     sources = SOURCES + [f for d in defines for f in VARIANT_SOURCES.get(d, [])]
-    with ThreadPoolExecutor(max_workers=8) as ex:
-        objs = list(ex.map(cc, sources))
-    r = subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib, *objs], capture_output=True, text=True)
-    if r.returncode:
-        raise RuntimeError(f"link failed:\n{r.stderr}")
+    objs, made = _objects(sources, os.path.join(CSRC, "build_" + tag), defines, force, verbose)
+    _run(lib, objs, [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib, *objs], "link", force or made, verbose)
     return lib
 
 
