@@ -13,21 +13,13 @@ LIB = os.path.join(HERE, "liba2v_hip.so")
 SOURCES = ["a2v_gemm.hip", "a2v_gemm_fast.hip", "a2v_gemm_p8.hip", "a2v_gemm_tn8.hip", "a2v_wgrad_slab.hip", "a2v_wgrad_sparse.hip", "a2v_conv_slab.hip", "a2v_conv_sparse.hip", "a2v_conv_dec.hip", "a2v_attn.hip", "a2v_linattn.hip", "a2v_qknorm.hip", "a2v_norm.hip", "a2v_elem.hip", "a2v_sinc.hip", "a2v_mixup.hip", "a2v_mask.hip", "a2v_conv_strided.hip", "a2v_split.hip"]
 # -amdgpu-mfma-vgpr-form: MFMA accumulators stay in arch VGPRs (no kernel here needs > 256 registers), which removes the
 # v_accvgpr_read/write copies around every VALU use of an accumulator (softmax, epilogues: 96 of 417 VALU per attention step)
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-mllvm", "-amdgpu-mfma-vgpr-form"]
-FLAGS += os.environ.get("A2V_HIPCC_FLAGS", "").split()      # extra -D switches of experiment builds (same-box A/B with tools/build_prev.sh)
-# a2v_attn.hip without the SLP vectoriser: paired into v_pk_fma_f32 the ALiBi term loses the |.| source modifier (one extra
-# v_and per score), and packed fp32 ops cost more issue time between MFMAs than two plain ones
-FILE_FLAGS = {"a2v_attn.hip": ["-fno-slp-vectorize"]}
-# No packed fp32 arithmetic: some forms of v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32, which -O3 makes of ordinary float code by
-# itself, have given wrong results on these cards now and then (hipcc's host pass warns that it does not know the feature: harmless).
-# Two files keep the code generation that their hand-counted waits and register budgets were written against: without packed
-# epilogues a2v_gemm_p8.hip drains its DMA pipeline in the K loop and spills in three variants, a2v_conv_dec.hip spills in one
-# (tests/test_abi.py holds both to neither).
+# No packed fp32 arithmetic in any file: some forms of v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32, which -O3 makes of ordinary float code
+# by itself, have given wrong results on these cards now and then (hipcc's host pass warns that it does not know the feature: harmless).
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-KEEPS_PACKED = ("a2v_gemm_p8.hip", "a2v_conv_dec.hip")
-for _s in SOURCES:
-    if _s not in KEEPS_PACKED:
-        FILE_FLAGS[_s] = NO_PACKED + FILE_FLAGS.get(_s, [])
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-mllvm", "-amdgpu-mfma-vgpr-form", *NO_PACKED]
+FLAGS += os.environ.get("A2V_HIPCC_FLAGS", "").split()      # extra -D switches of experiment builds (same-box A/B with tools/build_prev.sh)
+# a2v_attn.hip without the SLP vectoriser: what it pairs up costs more instructions between MFMAs than two plain ones
+FILE_FLAGS = {"a2v_attn.hip": ["-fno-slp-vectorize"]}
 # sources that only experiment libraries carry, by the -D switch that asks for them (never part of the product build):
 #   python -m animal2vec_amd.build --variant w2 -DA2V_W2     -> liba2v_hip_w2.so with the 256 x 128 two-per-CU NT kernel (round 4's
 #   negative result, profiles/r04_w2_experiment.txt), switched on with a2v_debug_set(25, 2)

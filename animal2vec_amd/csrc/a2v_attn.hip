@@ -695,9 +695,7 @@ __global__ __launch_bounds__(256, (QB == 2 && !DROP && !MD) ? 3 : 1) void attn_f
           f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < HD / 32; ++ks) acc = A2V_MFMA_16x16x32(kf[ks], qf[b][ks], acc, 0, 0, 0);
-          // acc + c_rel |pos_q - pos_k| = v_sub + one v_fma with the |.| source modifier.  This file is built with
-          // -fno-slp-vectorize: paired into v_pk_fma_f32 (no modifiers) the abs costs a separate v_and per element and the
-          // packed op more issue time next to MFMAs than two plain fmas (MI355X_MICROARCH.md cycle constants).
+          // acc + c_rel |pos_q - pos_k| = v_sub + one v_fma with the |.| source modifier
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[b][j][r] = __builtin_fmaf(__builtin_fabsf(pos_q[b] - pk[r]), c_rel, acc[r]);
         }

@@ -240,9 +240,8 @@ __device__ __forceinline__ float gelu_with_grad(float x, float& grad) {
   grad = fmaf(x * 0.39894228040143268f, e, 0.5f + copysignf(q, x));
   return fmaf(fabsf(x), q, 0.5f * x);
 }
-// The same for a PAIR of values in packed fp32 arithmetic (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32: two lanes' worth of
-// FMAs per issue slot; only v_rcp / v_exp and the sign / magnitude bit operations stay per component).  Same formulas, same
-// constants, same operation order as gelu_with_grad: bit-identical results.
+// The same for a PAIR of values, step by step side by side.  Same formulas, same constants, same operation order as gelu_with_grad:
+// bit-identical results.
 typedef float a2v_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ a2v_f32x2 gelu_with_grad2(a2v_f32x2 x, a2v_f32x2& grad) {
 #ifdef A2V_EXP_NOGELU

@@ -152,9 +152,11 @@ __global__ __launch_bounds__(256) void conv_dec_kernel(GemmArgs g, int nW, int f
     int clip_, t0_;
     block_pos(blk, clip_, t0_);
     const int t0 = t0_ - a.pad;
+    int tid_ = tid;                                   // opaque: places of the slab kept across the block loop would spill
+    asm volatile("" : "+v"(tid_));
 #pragma unroll
     for (int u = 0; u < CD_NLD; ++u) {
-      const int idx = tid + 256 * u;
+      const int idx = tid_ + 256 * u;
       const int row = idx / RCH, ch = idx - row * RCH;
       const bool ok = (unsigned)(t0 + row) < (unsigned)a.T_in;
       const cd_u32x4 z = {0u, 0u, 0u, 0u};

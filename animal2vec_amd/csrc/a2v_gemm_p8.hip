@@ -509,17 +509,17 @@ __global__ __launch_bounds__(512) void gemm_nt_bf16_p8_kernel(GemmArgs g, int st
     // atomic had returned, the stale copy came back afterwards: repeating tile ids, a launch that never ends).  In the epilogue the
     // 64 fragment registers are free; tests/test_abi.py still checks in the ISA that nothing touches the register in between.
     if (dynamic && tid == 0) {
-      const unsigned one = 1u, zoff = 0u;
+      unsigned one, zoff;                      // (constants of their own: as C++ ones they live, and spill, across the K loop)
+      asm volatile("v_mov_b32 %0, 1\n\tv_mov_b32 %1, 0" : "=v"(one), "=v"(zoff));
       // s_nop 4: the pointer's SGPRs may have just been restored by v_readlane (SGPR spill); a VMEM instruction reading an
       // SGPR written by VALU needs 5 wait states, which the compiler only inserts around instructions it can see
       asm volatile("s_nop 4\n\tglobal_atomic_add %0, %1, %2, %3 sc0" : "=v"(fetched) : "v"(zoff), "v"(one), "s"(&g_p8_ctr[xcd]) : "memory");
     }
-    // lane-derived values are re-formed in the epilogue from an opaque copy of the lane id.  The 8-bit-derivative fc1 flavour needs
-    // one register more than the bf16 one at the 256-row tile (a second per-lane store offset): there `lane` itself was spilled
-    // across the K loop and reloaded behind a full vmcnt(0) -- the tile claim's round trip -- so that flavour re-reads the hardware
-    // lane id instead (volatile asm: as builtins the two instructions are loop invariant and hoisted in front of the tile loop)
+    // lane-derived values are re-formed in the epilogue from an opaque copy of the lane id.  The fixed flavours have no register to keep `lane`
+    // in at the 256-row tile: it was spilled across the K loop and reloaded behind a full vmcnt(0) -- the tile claim's round trip -- so they
+    // re-read the hardware lane id (volatile asm: as builtins the two instructions are loop invariant and hoisted in front of the tile loop)
     int le = lane;
-    if constexpr (FX > 0 && (FX & F_DACT8) != 0 && (FX & F_STORE_PRE) != 0)
+    if constexpr (FX > 0)
       asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(le));
     else
       asm volatile("" : "+v"(le));
@@ -581,6 +581,8 @@ __global__ __launch_bounds__(512) void gemm_nt_bf16_p8_kernel(GemmArgs g, int st
             if (need_r) {
               float h[8];
               Vec8<float>::load(Rt + (long long)row * g.ldr + cl, h);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) asm volatile("" :: "v"(h[q]));       // consumed on every path (see the staged form below)
               if (flags & F_RES) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) v[q] += h[q];

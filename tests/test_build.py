@@ -49,3 +49,22 @@ def test_a_file_without_a_record_of_its_flags_is_built_again(build):
     ran(lambda: B.build(verbose=False))
     os.remove(src / "build" / "one.o.cmd")
     assert ran(lambda: B.build(verbose=False)) == ["one.hip", "link"]
+
+
+def test_no_file_is_compiled_with_packed_fp32_arithmetic(tmp_path):
+    """every source of the libraries takes the flag, and what the compiler makes of the two files with hand-counted register budgets, which
+    once went without, has none"""
+    import re
+    import shutil
+    import subprocess
+    from animal2vec_amd import build as B
+    for s in B.SOURCES:
+        assert "-packed-fp32-ops" in [*B.FLAGS, *B.FILE_FLAGS.get(s, [])], s
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not available")
+    for src in ("a2v_gemm_p8.hip", "a2v_conv_dec.hip"):
+        out = tmp_path / (src + ".s")
+        subprocess.run([hipcc, *B.FLAGS, *B.FILE_FLAGS.get(src, []), "-S", "--cuda-device-only", os.path.join(B.CSRC, src), "-o", str(out)], check=True, capture_output=True)
+        found = re.findall(r"\bv_pk_(?:add|mul|fma)_f32\b", out.read_text())
+        assert not found, (src, len(found))

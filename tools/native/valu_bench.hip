@@ -140,39 +140,6 @@ __global__ __launch_bounds__(256) void valu_kernel(unsigned long long* __restric
   if ((threadIdx.x & 63) == 0) stamps[(size_t)blockIdx.x * 4 + (threadIdx.x >> 6)] = t1 - t0;
 }
 
-// 64-bit register pairs: packed fp32
-#define OP8P(STR)                                                                                                              \
-  asm volatile(STR(0) STR(1) STR(2) STR(3) STR(4) STR(5) STR(6) STR(7)                                                         \
-               : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]), "+v"(p[4]), "+v"(p[5]), "+v"(p[6]), "+v"(p[7])                \
-               : "v"(px), "v"(py))
-#define P_FMA(n) "v_pk_fma_f32 %" #n ", %" #n ", %8, %9\n"
-#define P_MUL(n) "v_pk_mul_f32 %" #n ", %" #n ", %8\n"
-#define P_ADD(n) "v_pk_add_f32 %" #n ", %" #n ", %8\n"
-typedef float f2 __attribute__((ext_vector_type(2)));
-template <int OP>
-__global__ __launch_bounds__(256) void pk_kernel(unsigned long long* __restrict__ stamps, unsigned* __restrict__ sink, int loops) {
-  f2 p[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p[i] = (f2){1.0f + threadIdx.x * 1e-6f, 0.5f + i};
-  f2 px = {1.0000001f, 0.9999999f}, py = {1e-7f, -1e-7f};
-  __syncthreads();
-  const unsigned long long t0 = __builtin_amdgcn_s_memtime();
-  for (int l = 0; l < loops; ++l) {
-#pragma unroll
-    for (int k = 0; k < REP / 8; ++k) {
-      if constexpr (OP == 0) OP8P(P_FMA);
-      if constexpr (OP == 1) OP8P(P_MUL);
-      if constexpr (OP == 2) OP8P(P_ADD);
-    }
-  }
-  const unsigned long long t1 = __builtin_amdgcn_s_memtime();
-  float acc = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) acc += p[i][0] + p[i][1];
-  if (acc == 12345.678f) sink[0] = 1;
-  if ((threadIdx.x & 63) == 0) stamps[(size_t)blockIdx.x * 4 + (threadIdx.x >> 6)] = t1 - t0;
-}
-
 static unsigned long long* d_st; static unsigned* d_sink;
 template <typename K>
 static double run(K kern, int W, int loops) {
@@ -212,6 +179,5 @@ int main() {
   { printf("%-28s", "exp + fma (x 1/2)"); for (int W = 1; W <= 4; ++W) printf(" %8.2f", run(valu_kernel<40>, W, loops) / 2); printf("\n"); }
   { printf("%-28s", "exp + add + mul + and (x 1/4)"); for (int W = 1; W <= 4; ++W) printf(" %8.2f", run(valu_kernel<41>, W, loops) / 4); printf("\n"); }
   { printf("%-28s", "mul_lo + add + mul + and (1/4)"); for (int W = 1; W <= 4; ++W) printf(" %8.2f", run(valu_kernel<42>, W, loops) / 4); printf("\n"); }
-  ROW("v_pk_fma_f32 (2 per lane)", pk_kernel<0>) ROW("v_pk_mul_f32 (2 per lane)", pk_kernel<1>) ROW("v_pk_add_f32 (2 per lane)", pk_kernel<2>)
   return 0;
 }
