@@ -169,9 +169,10 @@ template <typename T, int HD> struct LinTile {
 };
 __device__ __forceinline__ int lin_channel(int t, int g, int i) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i; }         // of row 4 g + i of tile t
 // 16 bytes of each lane from base + off to lds + 16 lane, without a register in between.  In asm, so that the compiler does not wait for them in
-// front of every read from LDS: what waits is lin_wait, with the number of memory operations that are surely younger.
+// front of every read from LDS: what waits is lin_wait, with the number of memory operations that are surely younger.  (m0 cannot be named as
+// clobbered, and nothing else here uses it: the tests hold the compiled kernels to that, and to the number of younger operations.)
 __device__ __forceinline__ void lin_dma(const char* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
 // the lane, read again where it is needed: paths that are rarely taken keep nothing in registers for it
 __device__ __forceinline__ int lin_lane() {
@@ -537,11 +538,11 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
 #pragma unroll
           for (int k = 0; k < L::IN; ++k) vf[k][i] = ok ? vf[k][i] : (__bf16)0.f;
         }
-        row = min(row, __shfl_xor(row, 16, 64));
-        row = min(row, __shfl_xor(row, 32, 64));
+        row = min(row, __builtin_amdgcn_ds_bpermute((lane ^ 16) << 2, row));
+        row = min(row, __builtin_amdgcn_ds_bpermute((lane ^ 32) << 2, row));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                            // (of the channel and the two rows that an accumulator holds)
-          const int r0 = __shfl(row, 4 * g + i, 64);
+          const int r0 = __builtin_amdgcn_ds_bpermute((4 * g + i) << 2, row);
           if (fr >= r0) acc[0][i] = __builtin_nanf("");
           if (16 + fr >= r0) acc[1][i] = __builtin_nanf("");
         }
