@@ -29,7 +29,7 @@
 #include <type_traits>
 
 typedef __attribute__((address_space(3))) s16x4 la_lds_s16x4;
-// bfloat16 in both libraries: scores and states have its range, not half's
+// bfloat16 in both libraries: parts of scores and states need its range, not half's
 typedef __attribute__((ext_vector_type(2))) __bf16 lb2;
 typedef __attribute__((ext_vector_type(4))) __bf16 lb4;
 typedef __attribute__((ext_vector_type(8))) __bf16 lb8;
@@ -236,11 +236,11 @@ __device__ __forceinline__ float lin_log2(const float* slopes, int h) {
 __device__ __forceinline__ float lin_uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 __device__ __forceinline__ float lin_pow(float l2, int n) { return __builtin_amdgcn_exp2f(l2 * (float)n); }
 
-// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 212 us, 4.95 TB/s, where a large copy reaches 5.2 -- memory.
-// The backward of 192 clips of 140 rows: 0.6 us for a chunk and CU, the vector pipe busy for 59 % of it and the matrix pipe for 35 %; a chunk is
-// a chain of LDS reads, matrix and vector steps of 2 us, and four waves to a SIMD do not hide all of it.  A recording reads k and v twice, and
-// a long backward's dq, which runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from memory
-// instead of 4.
+// What bounds it (16 heads of 64 channels, 16-bit).  64 clips of 2000 rows, 1049 MB: 215 us, 4.87 TB/s, where a large copy reaches 5.2 -- memory.
+// The backward of 192 clips of 140 rows: 0.74 us for a chunk and CU, the vector pipe busy for 65 % of it and the matrix pipe for 49 %; a chunk is
+// a chain of LDS reads, matrix and vector steps of 2 us and more, and four waves to a SIMD do not hide all of it.  A recording reads k and v twice,
+// and a long backward's dq, which runs forward in time, shares nothing in the L2 with dk and dv, which run backwards: 7 operand reads from
+// memory instead of 4.
 // Registers: 128 with 16-bit operands, four waves to a SIMD; 32-bit ones take 166, three waves (two: 90 us against 84 for the training pair
 // of 2 x 2000 rows in fp32), with 128 channels two.
 //
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(HD * HEADS * 4, LinT<T>::IN == 1 ? 4 : HD == 128 ? 
 // element (any order of them: the waves' register image), eight loads in flight.  The part of `first` is added by the kernel that starts
 // from it.  A group of workgroups takes a sequence; of packed ones each that has something to scan, which reaches a multiple of LIN_INLINE
 // segments of rows: the group of the first such row looks for the sequence around it, so there are few groups however many sequences there
-// are.  (Short ones alone pay the launch, 4.8 us with 37 as with 10000 of them: their lengths are on the device.)
+// are.  (Short ones alone pay the launch, 4.8 us: their lengths are on the device.)
 __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs a, int HH) {
   const int per = a.H * HH / 256, group = blockIdx.x / per;
   const int i = (blockIdx.x - group * per) * 256 + threadIdx.x, h = i / HH;    // element of (H, HD, HD); HD * HD % 256 == 0
@@ -806,11 +806,10 @@ static void lin_launch_heads(const LinArgs& a, const LinPlan& p, hipStream_t str
 }
 // A head's 16-bit row is 64 or 128 bytes.  Four or two neighbouring heads to a workgroup read and write 256 at a time, which is worth more to
 // the memory than the larger workgroup costs, except where the card is not full of them or the kernel waits for its own steps:
-//   64 channels   64 x 2000 rows 212 us against 228, one recording 302 against 326; but 48 x 2000 rows (384 workgroups) 173 against 165, one clip
-//                 18.8 against 16.4, the training pair of 140-row clips 168 against 161 (its forward alone 50 against 48), packed shared heads 120
-//                 against 101
-//   32 channels   64 x 2000 rows 210 us against 299, the training pairs of 140-row clips 152 against 172 and of 4 x 11025 rows 329 against 455;
-//                 of 2 x 2000 rows 49 against 47
+//   64 channels   64 x 2000 rows 221 us against 245, one recording 305 against 341; but 48 x 2000 rows (384 workgroups) 182 against 170, one clip
+//                 19.5 against 16.9, the training pair of 140-row clips 194 against 181 (its forward alone 58 against 57)
+//   32 channels   64 x 2000 rows 216 us against 296, the training pairs of 140-row clips 169 against 193 and of 4 x 11025 rows 352 against 463;
+//                 of 2 x 2000 rows 53 against 48
 static bool lin_wide(const LinArgs& a, int HD, int heads) {
   if (heads == 1 || a.HK % heads || a.rep > 1 || (HD > 32 && a.roles > 1)) return false;
   if ((long long)a.slots * a.HK / heads < (HD > 32 ? LIN_WGS / 2 : LIN_WGS / 4)) return false;
@@ -838,7 +837,7 @@ static void lin_launch(int dtype, const LinArgs& a, const LinPlan& p, int HD, hi
 static int lin_dtype(int dtype) {
   if (dtype != A2V_F32 && dtype != A2V_BF16) return A2V_ERR_DTYPE;
 #ifdef A2V_ELT_F16
-  if (dtype == A2V_BF16) return A2V_ERR_UNSUPPORTED;             // states and scores have bf16's range, not half's (65504)
+  if (dtype == A2V_BF16) return A2V_ERR_UNSUPPORTED;             // (a half operand would be two bfloat16 parts: not built)
 #endif
   return A2V_OK;
 }

@@ -835,7 +835,7 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, inv_freq, pos=Non
 def _linear_attention_checks(what, q, k, v, slopes, state, cu_seqlens):
     """-> B, S, H, HK, HD"""
     if _HALF and q.dtype == torch.float16:
-        raise TypeError(f"{what}: not built for float16 (a state does not fit its range); use bfloat16 or float32")
+        raise TypeError(f"{what}: not built for float16 (the products take bfloat16 operands); use bfloat16 or float32")
     _heads(f"{what}: q", q, 4)
     _heads(f"{what}: k", k, 4, q)
     _heads(f"{what}: v", v, 4, q)
@@ -856,7 +856,8 @@ def _linear_attention_checks(what, q, k, v, slopes, state, cu_seqlens):
 def linear_attention_fwd(q, k, v, slopes, *, scale=None, state=None, cu_seqlens=None, out=None, want_state=False):
     """S_t = exp(-slopes[h]) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t  -> out (N,S,H,HD), state behind the last row or None.
 
-    q (N,S,H,HD), k, v (N,S,HK,HD) bf16 or fp32, views of a packed projection among them; HK divides H.  slopes (H) fp32 >= 0.
+    q (N,S,H,HD), k, v (N,S,HK,HD) bf16 or fp32, views of a packed projection among them; HK divides H.  slopes (H) fp32 >= 0, constants.
+    A row sees itself and the rows in front of it; t counts rows of the buffer (kept frames with gaps decay by their number, not by time).
     scale: default HD^-0.5.  state (B,H,HD,HD) fp32: what the sequences start from (None: nothing), never changed.
     cu_seqlens (B+1) int32 on the device: q, k, v are (1,T,heads,HD) and sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1], which may
     be none; rows outside every sequence are zeros in a result of this call's own and left as they were in the caller's `out`.
@@ -890,6 +891,7 @@ def linear_attention_fwd(q, k, v, slopes, *, scale=None, state=None, cu_seqlens=
 
 def linear_attention_bwd(q, k, v, slopes, d_out, *, scale=None, state=None, d_state=None, cu_seqlens=None, dq=None, dk=None, dv=None):
     """-> dq, dk, dv and the gradient of `state` (None without one).  d_state: gradient of the state behind the last row, or None.
+    slopes get no gradient: a model that learns them (or a scale of them) lacks that term.
     dq, dk, dv: all three (views of a packed gradient, for instance) or none; rows outside every sequence as in linear_attention_fwd.
     Gradients of a shared k / v head are summed over its heads in fp32; nothing here depends on the order of arrival."""
     what = "linear_attention_bwd"

@@ -207,16 +207,18 @@ int a2v_qk_norm_rope_bwd(int dtype, const void* dq_out, const void* dk_out, cons
                          const int* sections, int interleaved, float eps, int N, int S, int H, int HK, int HD, void* ws, size_t ws_bytes,
                          a2v_stream_t stream);
 size_t a2v_qk_norm_rope_workspace(int N, int S, int H, int HK, int HD);
-/* S_t = exp(-slopes[h]) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t;  slopes (H) fp32, >= 0 (infinity: only the row itself).
+/* S_t = exp(-slopes[h]) S_{t-1} + k_t v_t^T,  out_t = scale S_t^T q_t;  slopes (H) fp32, >= 0 (infinity: only the row itself), constants: the
+ * backward pass gives no gradient for them.  A row sees itself and the rows in front of it, and t counts rows of the buffer: where kept
+ * frames have gaps in time, the decay is not that of the time between them.
  * state / state_out (B, H, HD, HD) fp32 [channel of k][channel of v], before the first and behind the last row, either may be NULL;
  * they may not overlap (every part of a long sequence starts from the former).
  * cu_seqlens NULL: B sequences of S rows.  Else the tensors have S rows (sequence strides unused), sequence b is rows
  * cu_seqlens[b] .. cu_seqlens[b + 1] (B + 1 int32 on the device, ascending; a sequence may be empty: its state is handed on).  Rows
  * outside every sequence are left alone, or set to 0 with zero_outside.  Offsets outside [0, S] are clamped.
  * ws: a2v_linear_attention_workspace() bytes (0 where the axis is not split), 16-byte aligned; used by this call only.
- * dtype A2V_F32 or A2V_BF16; liba2v_hip_f16.so refuses its 16-bit type (A2V_ERR_UNSUPPORTED: a state does not fit half's range).
+ * dtype A2V_F32 or A2V_BF16; liba2v_hip_f16.so refuses its 16-bit type (A2V_ERR_UNSUPPORTED: the products take bfloat16 operands, not built).
  * A value that is not finite reaches what the formula says: its own row and those behind it (gradients of k and v: in front of it).  What
- * would be infinite may be NaN.
+ * would be infinite may be NaN, and fp32 values beyond bfloat16's range (3.39e38) count as infinite.
  * Limits, else A2V_ERR_ARG: fewer than 2^30 rows, rows less than 64 MiB apart, H / HK <= 1024, H HD HD < 2^28, fewer
  * than 2^31 / 3 / H segments. */
 int a2v_linear_attention_fwd(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, const float* slopes,
